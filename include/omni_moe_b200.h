@@ -521,6 +521,28 @@ OMNI_API int omni_router_norm_bwd(const float *dscores, const int32_t *indices, 
                          void *dlogits, void *scratch, size_t scratch_bytes, int32_t *status,
                          void *stream);
 
+/*
+ * The whole eval-mode layer for a few tokens (at most omni_decode_max_tokens() = 64) in one kernel: router gates,
+ * BatchNorm fold, log-softmax, product-key top-k, routed experts, shared SwiGLU MLP and the final add
+ * (OmniMoE.forward, omni_moe/modules/omni_moe.py:60-106), for the decode steps of a serving program.
+ *   x [T, H], gate_w, up_w [I, H], down_w [H, I], router_x, router_y [sqrt_n, H], up_table, down_table
+ *   [num_experts, H]  bf16, row-major, 16-byte aligned;  H (<= 16384) and I multiples of 8
+ *   bn_scale, bn_shift [2*sqrt_n] fp32: normalised = logit * scale + shift (both NULL = identity)
+ *   y [T, H] bf16, may not overlap any input
+ *   workspace: omni_decode_workspace_bytes(...) bytes, 16-byte aligned, whose first 512 bytes were zero before the
+ *   first launch that uses it; every launch leaves them zero.  Launches that may overlap on the GPU (other streams,
+ *   captured graphs that replay beside each other) need a workspace each.
+ * The kernel is launched cooperatively (its blocks wait on one another; each wait is bounded and sets
+ * OMNI_ST_WAIT_TIMEOUT).  Run-to-run identical: no atomics on results.
+ */
+OMNI_API int omni_decode_max_tokens(void);
+OMNI_API size_t omni_decode_workspace_bytes(int num_tokens, int intermediate, int sqrt_n, int k);
+OMNI_API int omni_decode(const void *x, const void *gate_w, const void *up_w, const void *down_w, const void *router_x,
+                         const void *router_y, const void *up_table, const void *down_table, const float *bn_scale,
+                         const float *bn_shift, int num_tokens, int hidden, int intermediate, int sqrt_n, int k,
+                         int64_t num_experts, void *y, void *workspace, size_t workspace_bytes, int32_t *status,
+                         void *stream);
+
 #ifdef __cplusplus
 }
 #endif

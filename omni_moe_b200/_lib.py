@@ -91,6 +91,10 @@ SIGNATURES = {
     "omni_mlp_gate_up_router": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
                                         c_void_p, c_void_p, c_void_p, c_void_p]),
     "omni_mlp_down": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "omni_decode_max_tokens": (c_int, []),
+    "omni_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "omni_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                            c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -360,6 +360,21 @@ class OmniMoE(nn.Module):
         out = y.view(bsz, seq_len, h)
         return out if in_dtype == torch.bfloat16 else out.to(in_dtype)
 
+    def decode(self, hidden_states: torch.Tensor) -> torch.Tensor:
+        """The eval-mode forward of at most 64 tokens ``[B, S, H]`` as one kernel (:func:`omni_decode_func`): the decode
+        steps of a serving program.  The same definition as :meth:`forward`, another order of summation.  Allocates
+        only its output (and a per-stream workspace once), so it can be captured in a CUDA graph; inference only."""
+        from ..ops.decode import omni_decode_func
+        if self.training:
+            raise RuntimeError("decode() uses the running statistics of the router's BatchNorm: call eval() first")
+        _lib.require_cuda(hidden_states)
+        operands = self._operands()
+        if hidden_states.dim() != 3 or hidden_states.size(2) != self.hidden_size:
+            raise ValueError(f"hidden_states must be (batch, sequence, {self.hidden_size}), got {tuple(hidden_states.shape)}")
+        y = omni_decode_func(hidden_states.reshape(-1, self.hidden_size), *operands, self.top_k, *self._bn_fold_eval())
+        self.last_status = _lib.device_status(hidden_states.device)
+        return y.view(hidden_states.shape)
+
     def graphed(self, num_tokens: int, device=None) -> "GraphedOmniMoE":
         """Capture one eval-mode forward for ``num_tokens`` tokens in a CUDA graph."""
         return GraphedOmniMoE(self, num_tokens, device)

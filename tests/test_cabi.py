@@ -94,3 +94,21 @@ def test_module_state_dict_matches_reference_names():
     assert m.up_embed.weight.shape == (256, 64) and m.router_gate_x.weight.shape == (16, 64)
     with pytest.raises(ValueError):
         OmniMoE(OmniMoEConfig(64, 128, "gelu", 256, 4))
+
+
+def test_decode_rejections(lib):
+    # x .. down_table, bn_scale, bn_shift | tokens, hidden, intermediate, sqrt_n, k, experts | y, workspace, bytes, status, stream
+    def call(t=4, h=64, i=64, n=8, k=4, experts=64, bn=(None, None)):
+        return lib.omni_decode(*([None] * 8), *bn, t, h, i, n, k, experts, None, None, 0, None, None), lib.omni_last_error()
+
+    for kw, what in ((dict(t=65), b"num_tokens"), (dict(t=-1), b"num_tokens"), (dict(h=60), b"multiple of 8"), (dict(h=0), b"multiple of 8"),
+                     (dict(h=16392), b"at most 16384"), (dict(i=4), b"intermediate"), (dict(n=1025, experts=1 << 21), b"sqrt_n"),
+                     (dict(k=0), b"k must be"), (dict(k=129, n=16, experts=256), b"k must be"), (dict(k=5, n=2, experts=4), b"exceeds"),
+                     (dict(experts=63), b"tables"), (dict(bn=(16, None)), b"together"), (dict(), b"NULL")):
+        rc, msg = call(**kw)
+        assert rc < 0 and what in msg, (kw, msg)
+    assert call(t=0)[0] == 0  # nothing to do
+    assert lib.omni_decode_max_tokens() == 64
+    assert lib.omni_decode_workspace_bytes(65, 64, 8, 4) == 0
+    # counters, logits, coefficients and indices, activation
+    assert lib.omni_decode_workspace_bytes(3, 40, 5, 7) == 512 + 128 + 2 * 96 + 240
