@@ -543,6 +543,42 @@ OMNI_API int omni_decode(const void *x, const void *gate_w, const void *up_w, co
                          int64_t num_experts, void *y, void *workspace, size_t workspace_bytes, int32_t *status,
                          void *stream);
 
+/*
+ * Root-mean-square norm with the residual's addition: the pre-norm of a block whose second half is the layer
+ * (the reference has the layer alone; its model's norm is torch code).  For every row of `hidden` (1 .. 16384) values:
+ *   h = x + residual, rounded to the type (h = x without a residual: residual and h both NULL)
+ *   rstd = (mean(h^2) + eps)^(-1/2)      y = h * rstd * weight
+ *   codes, scales: MX blocks of y (see omni_mx_quantize; both NULL = not wanted), from the fp32 values of y
+ * x, residual, y, h have type dtype (OMNI_F32 / BF16 / F16), weight that type or fp32 (w_dtype).  ldx, ldr: row strides in
+ * elements; outputs are contiguous.  rstd [rows] fp32 or NULL: what the gradient needs beside h.  Any alignment;
+ * 16-byte pieces are used where rows allow.  y and h may not overlap inputs, except h == residual or h == x with the
+ * same row stride.
+ */
+OMNI_API int omni_rms_norm(const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *weight, int w_dtype,
+                           int dtype, int64_t rows, int hidden, float eps, void *y, void *h, float *rstd, void *codes,
+                           void *scales, void *stream);
+/*
+ * Its gradient: dx (= the gradient of x and of the residual) [rows, hidden] from dy, dh (gradient of h from elsewhere, or
+ * NULL) and the saved h, rstd; dweight [hidden] in w_dtype or NULL, summed over rows in a fixed order (no atomics), with
+ * omni_rms_norm_bwd_scratch_bytes() of scratch.
+ */
+OMNI_API size_t omni_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden);
+OMNI_API int omni_rms_norm_bwd(const void *dy, int64_t lddy, const void *dh, int64_t lddh, const void *h, int64_t ldh,
+                               const void *weight, int w_dtype, int dtype, const float *rstd, int64_t rows, int hidden,
+                               void *dx, void *dweight, void *scratch, size_t scratch_bytes, void *stream);
+
+/*
+ * MX blocks: 32 neighbours of a row share a power-of-two scale, each value is held as e4m3.
+ *   codes [rows, cols] e4m3 bytes;  scales [rows, ceil(cols / 32)] e8m0 bytes: byte b stands for 2^(b - 127), the
+ *   smallest (b >= 0) for which the block's largest finite magnitude is <= 448 * 2^(b - 127)
+ *   code = v / scale to nearest, ties to even; a value that is not finite becomes NaN and does not count for the scale
+ * omni_mx_dequantize writes the values the codes stand for (exact where the type's range holds them).  Outputs are contiguous.
+ */
+OMNI_API int omni_mx_quantize(const void *x, int64_t ldx, int dtype, int64_t rows, int64_t cols, void *codes, void *scales,
+                              void *stream);
+OMNI_API int omni_mx_dequantize(const void *codes, const void *scales, int64_t rows, int64_t cols, int dtype, void *out,
+                                void *stream);
+
 #ifdef __cplusplus
 }
 #endif

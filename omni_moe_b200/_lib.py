@@ -91,6 +91,13 @@ SIGNATURES = {
     "omni_mlp_gate_up_router": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
                                         c_void_p, c_void_p, c_void_p, c_void_p]),
     "omni_mlp_down": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "omni_rms_norm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int64, c_int, c_float, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "omni_rms_norm_bwd_scratch_bytes": (c_size_t, [c_int64, c_int]),
+    "omni_rms_norm_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p,
+                                  c_int64, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "omni_mx_quantize": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "omni_mx_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "omni_decode_max_tokens": (c_int, []),
     "omni_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "omni_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

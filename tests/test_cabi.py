@@ -112,3 +112,22 @@ def test_decode_rejections(lib):
     assert lib.omni_decode_workspace_bytes(65, 64, 8, 4) == 0
     # counters, logits, coefficients and indices, activation
     assert lib.omni_decode_workspace_bytes(3, 40, 5, 7) == 512 + 128 + 2 * 96 + 240
+
+
+def test_norm_and_mx_rejections(lib):
+    def norm(dtype=1, w=1, rows=4, n=64, eps=1e-6, res=(None, None), mx=(None, None)):
+        return lib.omni_rms_norm(None, n, res[0], n, None, w, dtype, rows, n, eps, None, res[1], None, *mx, None), lib.omni_last_error()
+
+    for kw, what in ((dict(dtype=3), b"dtype"), (dict(dtype=1, w=2), b"weight"), (dict(rows=-1), b"rows"), (dict(n=0), b"hidden"),
+                     (dict(n=16385), b"hidden"), (dict(eps=-1.0), b"eps"), (dict(eps=float("nan")), b"eps"), (dict(res=(16, None)), b"together"),
+                     (dict(mx=(None, 16)), b"together"), (dict(), b"NULL")):
+        rc, msg = norm(**kw)
+        assert rc < 0 and what in msg, (kw, msg)
+    assert norm(rows=0)[0] == 0
+    assert lib.omni_rms_norm(16, 63, None, 0, 16, 1, 1, 2, 64, 1e-6, 16, None, None, None, None, None) < 0
+    assert b"row strides" in lib.omni_last_error()
+    assert lib.omni_rms_norm_bwd(16, 64, None, 0, 16, 64, 16, 1, 1, 16, 2, 64, 16, 16, None, 0, None) < 0
+    assert b"scratch" in lib.omni_last_error()
+    assert lib.omni_mx_quantize(None, 4, 0, 2, 0, None, None, None) < 0 and b"cols" in lib.omni_last_error()
+    assert lib.omni_mx_quantize(16, 3, 0, 2, 4, 16, 16, None) < 0 and b"row stride" in lib.omni_last_error()
+    assert lib.omni_mx_dequantize(None, None, 2, 4, 0, None, None) < 0 and b"NULL" in lib.omni_last_error()
