@@ -25,6 +25,7 @@
 // No load in this file uses cluster multicast.
 #include <cstdlib>
 
+#include "mx.cuh"
 #include "tcgen05.cuh"
 
 namespace omni {
@@ -34,10 +35,13 @@ using namespace tc;
 constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, each draining half of the columns
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 
-enum { EPI_F32 = 0, EPI_SWIGLU = 1, EPI_RES = 2, EPI_SWIGLU_CLAMP = 3 };
+enum { EPI_F32 = 0, EPI_SWIGLU = 1, EPI_RES = 2, EPI_SWIGLU_CLAMP = 3, EPI_SWIGLU_MX = 4, EPI_SWIGLU_CLAMP_MX = 5 };
 // EPI_SWIGLU_CLAMP is EPI_SWIGLU with gate and up limited to [-limit, limit] before the activation; a
 // separate instantiation, so the kernels of the common no-clamp case are compiled without it.
-__host__ __device__ constexpr bool is_swiglu(int epi) { return epi == EPI_SWIGLU || epi == EPI_SWIGLU_CLAMP; }
+// The _MX forms also keep the gate | up pre-activations as MX blocks for the backward (pair kernel only).
+__host__ __device__ constexpr bool is_mx(int epi) { return epi == EPI_SWIGLU_MX || epi == EPI_SWIGLU_CLAMP_MX; }
+__host__ __device__ constexpr bool is_clamp(int epi) { return epi == EPI_SWIGLU_CLAMP || epi == EPI_SWIGLU_CLAMP_MX; }
+__host__ __device__ constexpr bool is_swiglu(int epi) { return epi == EPI_SWIGLU || epi == EPI_SWIGLU_CLAMP || is_mx(epi); }
 
 struct GemmArgs {
   int M, N, K;          // N: logical output columns (EPI_SWIGLU: activation columns; EPI_F32 dual: per-axis columns)
@@ -53,6 +57,8 @@ struct GemmArgs {
   int tma_logits;         // pair kernel: 1 = the fp32 router logits do too (tensor map tm_lg)
   void* gu_out;           // EPI_SWIGLU: if set, [M, 2N] bf16 that also receives the gate | up pre-activations
   int64_t ldgu;
+  uint8_t* mx_codes;      // _MX: [M, 2N] e4m3 codes of the gate | up pre-activations
+  uint8_t* mx_scales;     // _MX: [M, 2 ceil(N / 32)] e8m0 scales (the gate's blocks, then the up's)
   // router tile columns of the fused gate/up + router-gate launch (pair kernel, EPI_SWIGLU only)
   int router_tiles;       // tile columns holding router sub-keys (0 = none); they come first in tile order
   int router_n;           // sqrt_n; kernels without router tiles and with a transposed B: k_split (0 = one B matrix)
@@ -143,6 +149,38 @@ __device__ __forceinline__ void swiglu_chunk(const uint32_t (&ra)[32], const uin
   }
 }
 
+// MX block of 32 accumulators of one row (the columns [col0, col0 + 32) of one of the two matrices): a lane holds a whole
+// block, so its maximum needs no shuffle.  Columns from col_lim on are not stored; their accumulators are zero (the
+// tensor map fills weight rows outside the matrix with zeros) and do not count.  codes: this row's codes at col0; `wide`:
+// the whole block can be stored as one 32-byte sector.
+__device__ __forceinline__ void save_mx_block(const uint32_t (&r)[32], uint8_t* codes, uint8_t* scale, int col0, int col_lim, bool wide) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = fmaxf(top, mx::finite_abs(__uint_as_float(r[i])));
+  const int s = mx::exponent_of(top);
+  const float inv = mx::pow2(-s);
+  uint32_t p[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    p[q] = mx::encode4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]), inv);
+  if (wide) {
+    st256(codes, p);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (col0 + 8 * q < col_lim) *reinterpret_cast<uint2*>(codes + 8 * q) = make_uint2(p[2 * q], p[2 * q + 1]);
+  }
+  *scale = static_cast<uint8_t>(s + 127);
+}
+__device__ __forceinline__ void save_mx_chunk(const uint32_t (&ra)[32], const uint32_t (&rb)[32], int row, int col0, int col_lim, const GemmArgs& g) {
+  uint8_t* c = g.mx_codes + static_cast<int64_t>(row) * (2 * g.N) + col0;
+  const int blocks = (g.N + mx::kBlock - 1) / mx::kBlock;
+  uint8_t* s = g.mx_scales + static_cast<int64_t>(row) * (2 * blocks) + col0 / mx::kBlock;
+  const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.mx_codes) & 31) == 0;
+  save_mx_block(ra, c, s, col0, col_lim, wide);
+  save_mx_block(rb, c + g.N, s + blocks, col0, col_lim, wide);
+}
+
 // Drains this warp's share of one accumulator tile: its 32 rows (TMEM lane quarter) and the column
 // chunks [c_begin, c_begin + 32 * NCH).  The TMEM load of chunk i+1 and the residual fetch of
 // chunk i are in flight while chunk i-1 is converted and stored.
@@ -170,12 +208,15 @@ __device__ __forceinline__ void store_tile(uint32_t taddr, int row, int col_tile
     tmem_ld_wait(ra);
     if (is_swiglu(EPI)) {
       tmem_ld_wait(rb);
-      swiglu_chunk<EPI == EPI_SWIGLU_CLAMP>(ra, rb, g.limit, v);
+      swiglu_chunk<is_clamp(EPI)>(ra, rb, g.limit, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ra[i]);
     }
-    if (is_swiglu(EPI) && g.gu_out != nullptr && live) {
+    if constexpr (is_mx(EPI)) {
+      if (live) save_mx_chunk(ra, rb, row, col0, col_lim, g);
+    }
+    if (is_swiglu(EPI) && !is_mx(EPI) && g.gu_out != nullptr && live) {
       // training: keep the pre-activations for the backward (gate in columns [0, N), up in [N, 2N))
       __nv_bfloat16* og = reinterpret_cast<__nv_bfloat16*>(g.gu_out) + static_cast<int64_t>(row) * g.ldgu + col0;
       __nv_bfloat16* ou = og + g.N;
@@ -302,12 +343,15 @@ __device__ __forceinline__ void store_tile_tma(uint32_t taddr, int row0, int col
     tmem_ld_wait(ra);
     if (is_swiglu(EPI)) {
       tmem_ld_wait(rb);
-      swiglu_chunk<EPI == EPI_SWIGLU_CLAMP>(ra, rb, g.limit, v);
+      swiglu_chunk<is_clamp(EPI)>(ra, rb, g.limit, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ra[i]);
     }
-    if (is_swiglu(EPI) && g.gu_out != nullptr && live) {
+    if constexpr (is_mx(EPI)) {
+      if (live) save_mx_chunk(ra, rb, row, col0, col_lim, g);
+    }
+    if (is_swiglu(EPI) && !is_mx(EPI) && g.gu_out != nullptr && live) {
       __nv_bfloat16* og = reinterpret_cast<__nv_bfloat16*>(g.gu_out) + static_cast<int64_t>(row) * g.ldgu + col0;
       __nv_bfloat16* ou = og + g.N;
       if (full && (g.ldgu & 15) == 0 && (g.N & 15) == 0 && (reinterpret_cast<uintptr_t>(g.gu_out) & 31) == 0) {
@@ -1101,6 +1145,31 @@ extern "C" int omni_mlp_gate_up_limit(const void* x, const void* gate_w, const v
   OMNI_SET_TUNING(g);
   if (limit > 0.f) return launch_pair<EPI_SWIGLU_CLAMP, false>(ma, mg, mu, mg, mu, g, static_cast<cudaStream_t>(stream));
   return launch_pair<EPI_SWIGLU, false>(ma, mg, mu, mg, mu, g, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int omni_mlp_gate_up_save_mx(const void* x, const void* gate_w, const void* up_w, int64_t num_tokens, int hidden,
+                                        int intermediate, float limit, void* act, void* codes, void* scales, int32_t* status,
+                                        void* stream) {
+  OMNI_REQUIRE(num_tokens >= 0 && num_tokens < (int64_t(1) << 31) - 2 * BM, "num_tokens out of range");
+  OMNI_REQUIRE(hidden >= 8 && hidden % 8 == 0, "hidden must be a positive multiple of 8, got %d", hidden);
+  OMNI_REQUIRE(intermediate >= 8 && intermediate % 8 == 0, "intermediate must be a positive multiple of 8, got %d", intermediate);
+  OMNI_REQUIRE(limit >= 0.f, "limit must be >= 0 (0 = no clamp), got %g", static_cast<double>(limit));  // also refuses NaN
+  if (num_tokens == 0) return 0;
+  OMNI_REQUIRE(x && gate_w && up_w && act && codes && scales && status, "NULL argument");
+  OMNI_REQUIRE(aligned16(x) && aligned16(gate_w) && aligned16(up_w) && aligned16(act) && aligned16(codes), "pointers must be 16-byte aligned");
+  CUtensorMap ma, mg, mu;
+  if (int e = make_map(&ma, x, num_tokens, hidden, BM)) return e;
+  if (int e = make_map(&mg, gate_w, intermediate, hidden, 128)) return e;
+  if (int e = make_map(&mu, up_w, intermediate, hidden, 128)) return e;
+  GemmArgs g{};
+  g.M = static_cast<int>(num_tokens), g.N = intermediate, g.K = hidden, g.dual = 0;
+  g.tiles_m = ceil_div(g.M, 2 * BM);
+  g.tiles_n = g.tiles_n_axis = ceil_div(intermediate, 128);
+  g.out = act, g.ldo = intermediate, g.limit = limit, g.status = status;
+  g.mx_codes = static_cast<uint8_t*>(codes), g.mx_scales = static_cast<uint8_t*>(scales);
+  OMNI_SET_TUNING(g);
+  if (limit > 0.f) return launch_pair<EPI_SWIGLU_CLAMP_MX, false>(ma, mg, mu, mg, mu, g, static_cast<cudaStream_t>(stream));
+  return launch_pair<EPI_SWIGLU_MX, false>(ma, mg, mu, mg, mu, g, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int omni_mlp_gate_up_save(const void* x, const void* gate_w, const void* up_w, int64_t num_tokens, int hidden,
