@@ -136,8 +136,26 @@ def ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+def stream_ptr(index: int | None = None) -> int:
+    """The current stream of device ``index`` (default: the current device) as the integer the C ABI takes.  Straight from
+    the binding: building a ``torch.cuda.Stream`` object costs as much as a small kernel launch."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index)
+
+
+class _NoSwitch:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def on_device(index: int):
+    """Context in which CUDA device ``index`` is current: nothing at all where it is already."""
+    return _NO_SWITCH if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -42,7 +42,7 @@ def mlp_ckpt_backward(dy: torch.Tensor, x: Optional[torch.Tensor], codes: torch.
     dgu = torch.empty((t, 2 * i), **bf)
     act = torch.empty((t, i), **bf) if need_down else None
     dact = gemm(dy, down_weight, False, True, status=status)              # dy [T,H] @ Wd [H,I]
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev.index):
         _lib.check(lib.omni_swiglu_bwd_mx(codes.data_ptr(), scales.data_ptr(), dact.data_ptr(), t, i, limit, dgu.data_ptr(),
                                           _lib.ptr(act), _lib.stream_ptr()))
     if need_down:
@@ -51,7 +51,7 @@ def mlp_ckpt_backward(dy: torch.Tensor, x: Optional[torch.Tensor], codes: torch.
         if i % 64 == 0:
             # dx = dgate @ Wg + dup @ Wu: the two weight matrices as one B operand stacked along K
             dx = torch.empty((t, h), **bf)
-            with torch.cuda.device(dev):
+            with _lib.on_device(dev.index):
                 _lib.check(lib.omni_gemm_bf16_stacked_b(dgu.data_ptr(), 0, 2 * i, gate_weight.data_ptr(), up_weight.data_ptr(), i, h,
                                                         t, h, 2 * i, dx.data_ptr(), h, status.data_ptr(), _lib.stream_ptr()))
         else:
@@ -75,7 +75,7 @@ class MlpCkptFunction(torch.autograd.Function):
         y = torch.empty((t, h), device=dev, dtype=torch.bfloat16)
         if t:
             lib, status = _lib.load(), _lib.device_status(dev).data_ptr()
-            with torch.cuda.device(dev):
+            with _lib.on_device(dev.index):
                 st = _lib.stream_ptr()
                 _lib.check(lib.omni_mlp_gate_up_save_mx(xb.data_ptr(), wg.data_ptr(), wu.data_ptr(), t, h, i, limit, act.data_ptr(),
                                                         codes.data_ptr(), scales.data_ptr(), status, st))

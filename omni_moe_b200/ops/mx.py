@@ -36,6 +36,8 @@ def check_mx(codes: torch.Tensor, scales: torch.Tensor) -> None:
 
 def rows_of(x: torch.Tensor) -> torch.Tensor:
     """``x [..., C]`` as a matrix whose rows are contiguous and do not overlap (a view wherever its strides allow)."""
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     x = x.reshape(-1, x.size(-1))
     contiguous_rows = x.size(1) == 1 or x.stride(1) == 1
     return x if contiguous_rows and (x.size(0) <= 1 or x.stride(0) >= x.size(1)) else x.contiguous()
@@ -51,9 +53,10 @@ def mx_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows, cols = x.shape
     codes, scales = empty_mx(rows, cols, x.device)
     if rows and cols:
-        with torch.cuda.device(x.device):
+        index = x.get_device()
+        with _lib.on_device(index):
             _lib.check(_lib.load().omni_mx_quantize(x.data_ptr(), x.stride(0), code, rows, cols, codes.data_ptr(),
-                                                    scales.data_ptr(), _lib.stream_ptr()))
+                                                    scales.data_ptr(), _lib.stream_ptr(index)))
     return codes, scales
 
 
@@ -66,7 +69,8 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
     rows, cols = codes.shape
     out = torch.empty((rows, cols), device=codes.device, dtype=dtype)
     if rows and cols:
-        with torch.cuda.device(codes.device):
+        index = codes.get_device()
+        with _lib.on_device(index):
             _lib.check(_lib.load().omni_mx_dequantize(codes.data_ptr(), scales.data_ptr(), rows, cols, code, out.data_ptr(),
-                                                      _lib.stream_ptr()))
+                                                      _lib.stream_ptr(index)))
     return out

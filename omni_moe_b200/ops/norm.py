@@ -24,17 +24,17 @@ class RmsNormOutput(NamedTuple):
 def _forward(x, residual, weight, eps, quantize, keep):
     """x, residual: matrices with contiguous rows.  Returns y, h (None without a residual), codes, scales, rstd."""
     t, n = x.shape
-    dev = x.device
-    y = torch.empty((t, n), device=dev, dtype=x.dtype)
-    h = torch.empty((t, n), device=dev, dtype=x.dtype) if residual is not None else None
-    rstd = torch.empty(t, device=dev, dtype=torch.float32) if keep else None
-    codes, scales = empty_mx(t, n, dev) if quantize else (None, None)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = None if residual is None else torch.empty_like(y)
+    rstd = torch.empty(t, device=x.device, dtype=torch.float32) if keep else None
+    codes, scales = empty_mx(t, n, x.device) if quantize else (None, None)
     if t:
-        with torch.cuda.device(dev):
+        index = x.get_device()
+        with _lib.on_device(index):
             _lib.check(_lib.load().omni_rms_norm(
                 x.data_ptr(), x.stride(0), _lib.ptr(residual), residual.stride(0) if residual is not None else 0, weight.data_ptr(),
                 _lib.dtype_code(weight.dtype), _lib.dtype_code(x.dtype), t, n, eps, y.data_ptr(), _lib.ptr(h), _lib.ptr(rstd),
-                _lib.ptr(codes), _lib.ptr(scales), _lib.stream_ptr()))
+                _lib.ptr(codes), _lib.ptr(scales), _lib.stream_ptr(index)))
     return y, h, codes, scales, rstd
 
 
@@ -42,18 +42,17 @@ def rms_norm_backward(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Ten
                       need_weight_grad: bool = True):
     """``(dx, dweight)``: ``dx`` is the gradient of ``x`` and of the residual alike."""
     t, n = h.shape
-    dev = h.device
-    dx = torch.empty((t, n), device=dev, dtype=h.dtype)
+    dx = torch.empty_like(h, memory_format=torch.contiguous_format)
     if t == 0:
         return dx, torch.zeros_like(weight) if need_weight_grad else None
-    dw = torch.empty(n, device=dev, dtype=weight.dtype) if need_weight_grad else None
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        scratch = torch.empty(lib.omni_rms_norm_bwd_scratch_bytes(t, n), device=dev, dtype=torch.uint8) if need_weight_grad else None
+    dw = torch.empty_like(weight) if need_weight_grad else None
+    lib, index = _lib.load(), h.get_device()
+    with _lib.on_device(index):
+        scratch = torch.empty(lib.omni_rms_norm_bwd_scratch_bytes(t, n), device=h.device, dtype=torch.uint8) if need_weight_grad else None
         _lib.check(lib.omni_rms_norm_bwd(
             dy.data_ptr(), dy.stride(0), _lib.ptr(dh), dh.stride(0) if dh is not None else 0, h.data_ptr(), h.stride(0),
             weight.data_ptr(), _lib.dtype_code(weight.dtype), _lib.dtype_code(h.dtype), rstd.data_ptr(), t, n, dx.data_ptr(),
-            _lib.ptr(dw), _lib.ptr(scratch), scratch.numel() if scratch is not None else 0, _lib.stream_ptr()))
+            _lib.ptr(dw), _lib.ptr(scratch), scratch.numel() if scratch is not None else 0, _lib.stream_ptr(index)))
     return dx, dw
 
 
@@ -96,26 +95,29 @@ def omni_rms_norm_func(x: torch.Tensor, weight: torch.Tensor, residual: Optional
 
     Sums are fp32.  Differentiable in ``x``, ``residual`` and ``weight``; the weight's gradient is summed in a fixed order.
     """
-    _lib.require_cuda(x, weight, residual)
+    index = x.get_device()
+    if index < 0 or weight.get_device() != index or (residual is not None and residual.get_device() != index):
+        _lib.require_cuda(x, weight, residual)
+        raise RuntimeError(f"all tensors must be on {x.device}")
     _lib.dtype_code(x.dtype)
-    n = x.size(-1) if x.dim() else 0
+    shape = x.shape
+    n = shape[-1] if shape else 0
     if not 1 <= n <= MAX_HIDDEN:
-        raise ValueError(f"the last dimension must be in [1, {MAX_HIDDEN}], got shape {tuple(x.shape)}")
+        raise ValueError(f"the last dimension must be in [1, {MAX_HIDDEN}], got shape {tuple(shape)}")
     if weight.shape != (n,):
         raise ValueError(f"weight must be ({n},), got {tuple(weight.shape)}")
-    if weight.dtype not in (x.dtype, torch.float32):
+    if weight.dtype != x.dtype and weight.dtype != torch.float32:
         raise TypeError(f"weight must be {x.dtype} or float32, got {weight.dtype}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("the residual must have the shape and type of x")
-    if any(v is not None and v.device != x.device for v in (weight, residual)):
-        raise RuntimeError(f"all tensors must be on {x.device}")
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    shape = x.shape
     xr, rr, w = rows_of(x), None if residual is None else rows_of(residual), weight.contiguous()
-    if torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in (x, residual, weight)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         y, h, codes, scales = RmsNormFunction.apply(xr, rr, w, eps, bool(quantize))
     else:
-        y, h, codes, scales, _ = _forward(xr.detach(), None if rr is None else rr.detach(), w.detach(), eps, bool(quantize), False)
-    return RmsNormOutput(y.view(shape), x if h is None else h.view(shape), codes, scales)
+        y, h, codes, scales, _ = _forward(xr, rr, w, eps, bool(quantize), False)
+    if len(shape) != 2:
+        y, h = y.view(shape), None if h is None else h.view(shape)
+    return RmsNormOutput(y, x if h is None else h, codes, scales)

@@ -241,7 +241,7 @@ def test_refusals():
                      (dict(up=p["up"][:60], down=p["down"][:60]), "rows"), (dict(down=p["down"][:63]), "rows"),
                      (dict(wd=p["wd"][:, :56]), "down_weight"), (dict(scale=None), "together"),
                      (dict(scale=p["scale"][:15]), "float32 vectors"), (dict(shift=p["shift"].half()), "float32 vectors"),
-                     (dict(x=p["x"][0]), "matrices")):
+                     (dict(x=p["x"][0]), "matrix of tokens")):
         with pytest.raises(ValueError, match=what):
             call(p, **kw)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
