@@ -1049,6 +1049,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 using namespace omni;
 
+int omni::tc::tile_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int box_rows) {
+  return make_map(m, ptr, rows, cols, box_rows);
+}
+
 extern "C" int omni_router_gate(const void* x, const void* gate_x, const void* gate_y, int64_t num_tokens, int hidden,
                                 int sqrt_n, float* logits, int32_t* status, void* stream) {
   return omni::router_gate_if(x, gate_x, gate_y, num_tokens, hidden, sqrt_n, logits, nullptr, status, stream);

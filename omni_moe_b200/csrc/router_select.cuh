@@ -55,11 +55,6 @@ __device__ __forceinline__ float load_as_float(const void* base, int dtype, int6
   return __half2float(reinterpret_cast<const __half*>(base)[i]);
 }
 
-template <bool COHERENT>
-__device__ __forceinline__ float load_logit(const float* p) {
-  return COHERENT ? __ldcg(p) : __ldg(p);
-}
-
 // Small rows (at most 64 entries, two per lane): rank every entry by counting the entries that beat
 // it.  The entries are made distinct by packing (score key, ~index) into 64 bits, so the ranks are a
 // permutation; there is no cross-lane dependency chain, only broadcast reads of shared memory.
@@ -252,7 +247,6 @@ __device__ __forceinline__ void warp_select_sorted(const uint32_t (&key)[E], con
 // only serves small k can shrink it.
 template <int VPL, int CPL, int KCAP = kMaxK>
 struct WarpScratch {
-  static constexpr bool kCoherent = false;  // true in a kernel whose own launch writes the logits: no read-only cache
   static constexpr bool kAllSmall = (VPL == 2) && (CPL == 2);
   __align__(16) unsigned long long pack[kAllSmall ? 64 : kMaxK];  // ranking scratch
   uint32_t rk[CPL == 2 ? 64 : kMaxK], rf[CPL == 2 ? 64 : kMaxK];  // selected (score key, flat index) by rank
@@ -325,7 +319,7 @@ __device__ __forceinline__ unsigned select_axes_small(const TopkArgs& a, int64_t
 #pragma unroll
   for (int ax = 0; ax < 2; ++ax)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) v[ax][e] = (e * 32 + lane) < n ? load_logit<Scratch::kCoherent>(row + ax * n + e * 32 + lane) : -INFINITY;
+    for (int e = 0; e < 2; ++e) v[ax][e] = (e * 32 + lane) < n ? __ldg(row + ax * n + e * 32 + lane) : -INFINITY;
   if (a.bn_scale) {
     float sc[2][2], sh[2][2];
 #pragma unroll
@@ -431,7 +425,7 @@ __device__ __forceinline__ void select_token(const TopkArgs& a, int64_t t, Scrat
 #pragma unroll
       for (int e = 0; e < VPL; ++e) {
         const int c = e * 32 + lane;
-        v[e] = c < n ? load_logit<Scratch::kCoherent>(row + c) : -INFINITY;
+        v[e] = c < n ? __ldg(row + c) : -INFINITY;
       }
       if (a.bn_scale) {
         float sc[VPL], sh[VPL];

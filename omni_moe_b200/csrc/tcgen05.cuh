@@ -122,6 +122,17 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32
       : "r"(taddr)
       : "memory");
 }
+// The same for 16 columns, waited for.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 // Waits for this thread's outstanding tcgen05.ld.  The registers are passed through the statement
 // so that no use of them can be scheduled ahead of the wait.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
@@ -223,6 +234,10 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint16_t cta_mask
                ::"r"(bar), "h"(cta_mask)
                : "memory");
 }
+
+// Tensor map of a row-major bf16 matrix [rows, cols] with boxes of box_rows x 64 columns in the 128-byte swizzle
+// (defined in gemm_tcgen05.cu; 0 or the error code of fail()).
+int tile_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t cols, int box_rows);
 
 }  // namespace tc
 }  // namespace omni

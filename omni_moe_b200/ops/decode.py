@@ -96,7 +96,7 @@ def omni_decode_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
         lib = _lib.load()
         with _lib.on_device(index):
             stream = _lib.stream_ptr(index)
-            ws = _workspace(lib.omni_decode_workspace_bytes(t, i, n, k), index, stream)
+            ws = _workspace(lib.omni_decode_workspace_bytes(t, h, i, n, k), index, stream)
             _lib.check(lib.omni_decode(*pointers, _lib.ptr(bn_scale), _lib.ptr(bn_shift), t, h, i, n, k, experts, y.data_ptr(),
                                        ws.data_ptr(), ws.numel(), _lib.device_status(x.device).data_ptr(), stream))
     return y

@@ -249,3 +249,50 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="no backward"):
         call(p, x=p["x"].clone().requires_grad_())
     check(p, call(p))
+
+
+@pytest.mark.parametrize("t,h,i,n,k", [
+    (9, 4096, 8192, 64, 16),   # the ring form: 16, 32 and 64 token columns
+    (16, 4096, 8192, 30, 16),
+    (17, 1024, 4096, 64, 16),
+    (48, 2048, 8192, 256, 16),
+    (20, 64, 20000, 8, 4),     # more than 128 gate / up columns a block
+    (64, 128, 40000, 4, 4),
+    (18, 8, 8, 3, 2),          # fewer columns than blocks everywhere
+    (30, 264, 1000, 1000, 64),  # router rows of both axes in one tile
+    (25, 16, 264, 1024, 128),
+    (33, 8192, 520, 40, 20),
+])
+def test_ring_form(t, h, i, n, k):
+    p = make(t, h, i, n, k, t + h + i, table_std=0.1)
+    check(p, call(p))
+
+
+@pytest.mark.parametrize("t", [3, 20])
+@pytest.mark.parametrize("n,k", [(40, 12), (200, 16), (300, 64), (1024, 64)])
+def test_ties_go_to_the_lower_index(t, n, k):
+    """Sub-keys that come in equal pairs and fours: whole groups of scores are equal, inside and across the border of
+    the k best.  The selection is compared through the output of a layer whose MLP is zero."""
+    g = gen(n + t)
+    h = 64
+    p = make(t, h, 64, n, k, 11, table_std=0.5)
+    p["wd"].zero_()
+    p["kx"], p["ky"] = p["kx"][torch.arange(n) // 2 * 2], p["ky"][torch.arange(n) // 4 * 4]
+    p["scale"] = p["shift"] = None
+    x = p["x"].double()
+    z = [torch.log_softmax(x @ p[w].double().t(), 1) for w in ("kx", "ky")]
+    grid = (z[0][:, :, None] + z[1][:, None, :]).flatten(1)
+    # equal rows of a matrix product are equal whatever the summation, so the 64-bit scores tie exactly where fp32's do;
+    # a stable descending sort ranks them by index
+    # (in 64 bits equal sums of different parts would also be kept apart: nearer than 1e-5 is left to fp32)
+    order = torch.sort(grid, dim=1, descending=True, stable=True)
+    best, at = order.values[:, :k], order.indices[:, :k]
+    gaps = order.values[:, :k] - order.values[:, 1:k + 1]
+    clear = ~((gaps > 1e-12) & (gaps < 1e-5)).any(1)
+    dot = (p["up"][at].double() * x[:, None]).sum(2)
+    coef = best.exp() * dot / (1 + torch.exp(-dot))
+    terms = coef[:, :, None] * p["down"][at].double()
+    bound = 2 ** -8 * terms.sum(1).abs() + 1e-3 * terms.abs().sum(1) + 1e-7
+    assert clear.sum() >= t // 2
+    off = (call(p).double() - terms.sum(1)).abs()
+    assert (off <= bound)[clear].all()
