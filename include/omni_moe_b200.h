@@ -565,7 +565,8 @@ OMNI_API int omni_rms_norm(const void *x, int64_t ldx, const void *residual, int
 OMNI_API size_t omni_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden);
 OMNI_API int omni_rms_norm_bwd(const void *dy, int64_t lddy, const void *dh, int64_t lddh, const void *h, int64_t ldh,
                                const void *weight, int w_dtype, int dtype, const float *rstd, int64_t rows, int hidden,
-                               void *dx, void *dweight, void *scratch, size_t scratch_bytes, void *stream);
+                               void *dx, void *dweight, void *scratch, size_t scratch_bytes, int32_t *status,
+                               void *stream);
 
 /*
  * MX blocks: 32 neighbours of a row share a power-of-two scale, each value is held as e4m3.

@@ -95,7 +95,7 @@ SIGNATURES = {
                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "omni_rms_norm_bwd_scratch_bytes": (c_size_t, [c_int64, c_int]),
     "omni_rms_norm_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p,
-                                  c_int64, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                  c_int64, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "omni_mx_quantize": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "omni_mx_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "omni_mlp_gate_up_save_mx": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,

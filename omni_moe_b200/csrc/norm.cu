@@ -13,6 +13,7 @@
 // registers; one partial row per block goes to scratch and a second kernel adds the partial rows in block order (no
 // atomics: run-to-run identical).
 #include "mx.cuh"
+#include "tcgen05.cuh"
 
 namespace omni {
 namespace {
@@ -211,12 +212,72 @@ struct NormBwdArgs {
   int warps, rpc;
   void* dx;
   float* partial;  // [blocks, H] or null
+  int32_t* status;
 };
 
+// The columns' sums of a block's row groups, added in group order.
+template <int VE, int V>
+__device__ __forceinline__ void put_partial(const NormBwdArgs& a, const float (&dw)[V][VE], float* s_dw, int tpr, int grp, int tid) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (i * tpr + tid) * VE;
+    if (c < a.H) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s_dw[grp * a.H + c + e] = dw[i][e];
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
+    float s = 0.f;
+    for (int q = 0; q < a.rpc; ++q) s += s_dw[q * a.H + c];
+    a.partial[static_cast<int64_t>(blockIdx.x) * a.H + c] = s;
+  }
+}
+
+// One row, held by its threads: adds to their columns' sums and writes dx.
+template <typename T, int VE, int V>
+__device__ __forceinline__ void bwd_row(const NormBwdArgs& a, const Pack<T, VE> (&ph)[V], const Pack<T, VE> (&pg)[V], const Pack<T, VE> (&pd)[V],
+                                        float rho, int64_t t, bool live, float (&dw)[V][VE], int tpr, int grp, int tid, float* s_sum) {
+  float dot = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (i * tpr + tid) * VE;
+    if (live && c < a.H) {
+      float w[VE];
+      load_weight<T, VE>(a.w, a.w_f32, c, w);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float g = to_f<T>(pg[i].v[e]), n = to_f<T>(ph[i].v[e]) * rho;
+        dw[i][e] = __fmaf_rn(g, n, dw[i][e]);
+        dot = __fmaf_rn(g * w[e], n, dot);
+      }
+    }
+  }
+  dot = row_sum(dot, a.warps, grp, tid >> 5, s_sum) / static_cast<float>(a.H);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (i * tpr + tid) * VE;
+    if (live && c < a.H) {
+      float w[VE];
+      load_weight<T, VE>(a.w, a.w_f32, c, w);
+      Pack<T, VE> o;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float n = to_f<T>(ph[i].v[e]) * rho;
+        float d = rho * __fmaf_rn(-n, dot, to_f<T>(pg[i].v[e]) * w[e]);
+        if (a.dh) d += to_f<T>(pd[i].v[e]);
+        o.v[e] = from_f<T>(d);
+      }
+      store_pack<T, VE>(static_cast<T*>(a.dx) + t * a.H + c, o);
+    }
+  }
+}
+
+// Rows straight into registers, one after the other: few rows, or rows that cannot be copied in 16-byte pieces.
 template <typename T, int VE, int V>
 __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const NormBwdArgs a) {
   __shared__ float s_sum[2 * 8 * 16];
-  extern __shared__ float s_dw[];  // [rpc, H]: the row groups' column sums
+  extern __shared__ __align__(16) uint8_t s_dyn[];
   const int tpr = a.warps * 32;
   const int grp = threadIdx.x / tpr, tid = threadIdx.x - grp * tpr;
   float dw[V][VE] = {};
@@ -241,56 +302,83 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const NormBwdArgs a) 
         if (live && c < a.H) pd[i] = load_pack<T, VE>(dh + c);
       }
     }
-    const float rho = live ? a.rstd[t] : 0.f;
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (i * tpr + tid) * VE;
-      if (live && c < a.H) {
-        float w[VE];
-        load_weight<T, VE>(a.w, a.w_f32, c, w);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float g = to_f<T>(pg[i].v[e]), n = to_f<T>(ph[i].v[e]) * rho;
-          dw[i][e] = __fmaf_rn(g, n, dw[i][e]);
-          dot = __fmaf_rn(g * w[e], n, dot);
-        }
-      }
-    }
-    dot = row_sum(dot, a.warps, grp, tid >> 5, s_sum + turn * 128) / static_cast<float>(a.H);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (i * tpr + tid) * VE;
-      if (live && c < a.H) {
-        float w[VE];
-        load_weight<T, VE>(a.w, a.w_f32, c, w);
-        Pack<T, VE> o;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float n = to_f<T>(ph[i].v[e]) * rho;
-          float d = rho * __fmaf_rn(-n, dot, to_f<T>(pg[i].v[e]) * w[e]);
-          if (a.dh) d += to_f<T>(pd[i].v[e]);
-          o.v[e] = from_f<T>(d);
-        }
-        store_pack<T, VE>(static_cast<T*>(a.dx) + t * a.H + c, o);
-      }
-    }
+    bwd_row<T, VE, V>(a, ph, pg, pd, live ? a.rstd[t] : 0.f, t, live, dw, tpr, grp, tid, s_sum + turn * 128);
   }
-  if (!a.partial) return;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = (i * tpr + tid) * VE;
-    if (c < a.H) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) s_dw[grp * a.H + c + e] = dw[i][e];
-    }
+  if (a.partial) put_partial<VE, V>(a, dw, reinterpret_cast<float*>(s_dyn), tpr, grp, tid);
+}
+
+// Many rows: the copy engine brings whole rows into a ring of shared-memory stages (rpc rows of h, dy and dh each), ahead
+// of the threads, so that the barrier of a row's sum leaves no gap in the traffic.  (16384 x 4096 bf16: rows into registers
+// 191 us, the next row's registers loaded ahead 140 us.)
+constexpr int kBwdStages = 3;
+template <typename T, int VE, int V>
+__global__ void __launch_bounds__(512) rms_norm_bwd_ring_kernel(const NormBwdArgs a) {
+  __shared__ float s_sum[2 * 8 * 16];
+  __shared__ __align__(8) uint64_t s_full[kBwdStages];
+  __shared__ int s_abort;
+  extern __shared__ __align__(16) uint8_t s_dyn[];  // stages of [3][rpc][H]; afterwards the row groups' column sums
+  const int tpr = a.warps * 32;
+  const int grp = threadIdx.x / tpr, tid = threadIdx.x - grp * tpr;
+  const uint32_t full = tc::smem_u32(s_full);
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < kBwdStages; ++i) tc::mbar_init(full + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
-    float s = 0.f;
-    for (int q = 0; q < a.rpc; ++q) s += s_dw[q * a.H + c];
-    a.partial[static_cast<int64_t>(blockIdx.x) * a.H + c] = s;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.rpc, first = static_cast<int64_t>(blockIdx.x) * a.rpc;
+  const uint32_t row_bytes = a.H * sizeof(T);
+  const int tensors = a.dh ? 3 : 2;
+  const auto fetch = [&](int64_t t0, int stage) {  // one thread
+    const int rows = static_cast<int>(a.T - t0 < a.rpc ? a.T - t0 : a.rpc);
+    const uint32_t bar = full + 8 * stage;
+    tc::mbar_arrive_expect_tx(bar, rows * tensors * row_bytes);
+    for (int q = 0; q < tensors; ++q) {
+      const T* src = static_cast<const T*>(q == 0 ? a.h : (q == 1 ? a.dy : a.dh));
+      const int64_t ld = q == 0 ? a.ldh : (q == 1 ? a.lddy : a.lddh);
+      for (int i = 0; i < rows; ++i)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         tc::smem_u32(s_dyn) + ((stage * 3 + q) * a.rpc + i) * row_bytes),
+                     "l"(src + (t0 + i) * ld), "r"(row_bytes), "r"(bar)
+                     : "memory");
+    }
+  };
+  if (threadIdx.x == 0)
+    for (int i = 0; i < kBwdStages; ++i)
+      if (first + i * step < a.T) fetch(first + i * step, i);
+  float dw[V][VE] = {};
+  int turn = 0, stage = 0;
+  uint32_t phase = 0;
+  for (int64_t t0 = first; t0 < a.T; t0 += step, turn ^= 1) {
+    const int64_t t = t0 + grp;
+    const bool live = t < a.T;
+    const float rho = live ? a.rstd[t] : 0.f;
+    // a wait that runs out (a defect) flags it and leaves: every thread sees the flag after the barrier
+    tc::mbar_wait(full + 8 * stage, phase, &s_abort, a.status);
+    Pack<T, VE> ph[V], pg[V], pd[V];
+    const T* base = reinterpret_cast<const T*>(s_dyn) + (static_cast<int64_t>(stage) * 3 * a.rpc + grp) * a.H;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (i * tpr + tid) * VE;
+      if (live && c < a.H) {
+        ph[i] = load_pack<T, VE>(base + c), pg[i] = load_pack<T, VE>(base + a.rpc * a.H + c);
+        if (a.dh) pd[i] = load_pack<T, VE>(base + 2 * a.rpc * a.H + c);
+      }
+    }
+    __syncthreads();  // the stage is read: it can be filled again
+    if (s_abort) break;
+    if (threadIdx.x == 0 && t0 + kBwdStages * step < a.T) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the reads above come before the copies' writes
+      fetch(t0 + kBwdStages * step, stage);
+    }
+    if (++stage == kBwdStages) stage = 0, phase ^= 1;
+    bwd_row<T, VE, V>(a, ph, pg, pd, rho, t, live, dw, tpr, grp, tid, s_sum + turn * 128);
   }
+  if (s_abort) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies that are still on their way land before the block leaves
+  }
+  __syncthreads();
+  if (a.partial) put_partial<VE, V>(a, dw, reinterpret_cast<float*>(s_dyn), tpr, grp, tid);
 }
 
 // dw[c] = the sum of the partial rows in block order: 32 columns x 8 slices of rows a block.
@@ -346,26 +434,35 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
   }
 }
 
+// Decoded values: a thread has VE neighbours of a row (16: a 16-byte piece of codes), a block of threads walks along
+// one row, the grid's second dimension over rows: no division.
 template <typename T, int VE>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             int64_t rows, int cols, T* out) {
   const int scols = (cols + mx::kBlock - 1) / mx::kBlock;
-  const int per_row = (cols + VE - 1) / VE;
-  const int64_t total = rows * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t t = i / per_row;
-    const int c = static_cast<int>(i - t * per_row) * VE;
-    const float sc = mx::pow2(static_cast<int>(scales[t * scols + c / mx::kBlock]) - 127);
-    Pack<T, VE> o;
-    if constexpr (VE == 8) {
-      const uint2 q = *reinterpret_cast<const uint2*>(codes + t * cols + c);
-      const float2 f0 = mx::decode2(q.x), f1 = mx::decode2(q.x >> 16), f2 = mx::decode2(q.y), f3 = mx::decode2(q.y >> 16);
-      o.v[0] = from_f<T>(f0.x * sc), o.v[1] = from_f<T>(f0.y * sc), o.v[2] = from_f<T>(f1.x * sc), o.v[3] = from_f<T>(f1.y * sc);
-      o.v[4] = from_f<T>(f2.x * sc), o.v[5] = from_f<T>(f2.y * sc), o.v[6] = from_f<T>(f3.x * sc), o.v[7] = from_f<T>(f3.y * sc);
+  const int c = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x) * VE;
+  if (c >= cols) return;
+#pragma unroll 2
+  for (int64_t t = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; t < rows; t += static_cast<int64_t>(gridDim.y) * blockDim.y) {
+    const uint8_t* p = codes + t * cols + c;
+    const float sc = mx::pow2(static_cast<int>(__ldg(scales + t * scols + c / mx::kBlock)) - 127);
+    if constexpr (VE == 16) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        Pack<T, 8> o;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f0 = mx::decode2(w[2 * half + e]), f1 = mx::decode2(w[2 * half + e] >> 16);
+          o.v[4 * e] = from_f<T>(f0.x * sc), o.v[4 * e + 1] = from_f<T>(f0.y * sc);
+          o.v[4 * e + 2] = from_f<T>(f1.x * sc), o.v[4 * e + 3] = from_f<T>(f1.y * sc);
+        }
+        store_pack<T, 8>(out + t * cols + c + 8 * half, o);
+      }
     } else {
-      o.v[0] = from_f<T>(mx::decode2(codes[t * cols + c]).x * sc);
+      out[t * cols + c] = from_f<T>(mx::decode2(*p).x * sc);
     }
-    store_pack<T, VE>(out + t * cols + c, o);
   }
 }
 
@@ -386,8 +483,8 @@ void row_shape(int64_t T, int H, int per_thread, int& per, int& warps, int& rpc)
   rpc = warps >= 8 ? 1 : 8 / warps;
   if (T < rpc) rpc = static_cast<int>(T);
 }
-// Many rows: more values a thread (fewer barriers, more bytes in flight a warp); few rows: 8, so that a row's loads are
-// spread over more warps.  Rows that move value by value need an address each: 8 as well.
+// Many rows: 16 values a thread (16384 x 4096 bf16 with residual and codes: 8 / 16 / 32 values 121 / 106 / 117 us); few
+// rows: 8, so that a row's loads are spread over more warps.  Rows that move value by value need an address each: 8 as well.
 constexpr int kManyRows = 1024;
 
 template <typename T>
@@ -397,7 +494,7 @@ int launch_norm(const NormArgs& a0, cudaStream_t st) {
   const bool vec = a.H % VE == 0 && at16(a.x) && at16(a.r) && at16(a.w) && at16(a.y) && at16(a.h) && at16(a.codes) &&
                    (a.ldx * sizeof(T)) % 16 == 0 && (a.ldr * sizeof(T)) % 16 == 0;
   int per;
-  row_shape(a.T, a.H, vec && a.T >= kManyRows ? 32 : 8, per, a.warps, a.rpc);
+  row_shape(a.T, a.H, vec && a.T >= kManyRows ? 16 : 8, per, a.warps, a.rpc);
   const int64_t blocks = ceil_div64(a.T, a.rpc);
   OMNI_REQUIRE(blocks < (int64_t(1) << 31), "too many rows");
   const dim3 grid(static_cast<unsigned>(blocks)), block(a.rpc * a.warps * 32);
@@ -413,18 +510,36 @@ int launch_norm(const NormArgs& a0, cudaStream_t st) {
   return check_launch("rms_norm_kernel");
 }
 
+// Two blocks a multiprocessor, fewer where a block would have less than four turns (each costs a partial row).
 int bwd_blocks(int64_t T, int rpc) {
-  const int64_t want = ceil_div64(T, rpc), most = 2 * static_cast<int64_t>(multiprocessors());
-  return static_cast<int>(want < most ? want : most);
+  const int64_t turns = ceil_div64(T, rpc), sms = multiprocessors();
+  int64_t blocks = turns / 4 < sms ? (turns < sms ? turns : sms) : turns / 4;
+  if (blocks > 2 * sms) blocks = 2 * sms;
+  return static_cast<int>(blocks);
 }
 
 template <typename T, int VE, int V>
 int launch_bwd(const NormBwdArgs& a, int blocks, cudaStream_t st) {
-  const size_t smem = a.partial ? sizeof(float) * a.rpc * a.H : 0;
+  const size_t sums = a.partial ? sizeof(float) * a.rpc * a.H : 0;
+  const dim3 block(a.rpc * a.warps * 32);
+  if constexpr (VE > 1) {
+    const size_t ring = static_cast<size_t>(kBwdStages) * 3 * a.rpc * a.H * sizeof(T);
+    if (a.T >= kManyRows && ring <= 110 * 1024) {
+      static OncePerDevice once;
+      if (once.first() && cudaFuncSetAttribute(rms_norm_bwd_ring_kernel<T, VE, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, 110 * 1024) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return fail(-2, "cannot raise the shared-memory limit of rms_norm_bwd_ring_kernel");
+      }
+      rms_norm_bwd_ring_kernel<T, VE, V><<<blocks, block, ring > sums ? ring : sums, st>>>(a);
+      return check_launch("rms_norm_bwd_ring_kernel");
+    }
+  }
   static OncePerDevice once;
-  if (once.first() && cudaFuncSetAttribute(rms_norm_bwd_kernel<T, VE, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMaxHidden) != cudaSuccess)
+  if (once.first() && cudaFuncSetAttribute(rms_norm_bwd_kernel<T, VE, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMaxHidden) != cudaSuccess) {
+    (void)cudaGetLastError();
     return fail(-2, "cannot raise the shared-memory limit of rms_norm_bwd_kernel");
-  rms_norm_bwd_kernel<T, VE, V><<<blocks, a.rpc * a.warps * 32, smem, st>>>(a);
+  }
+  rms_norm_bwd_kernel<T, VE, V><<<blocks, block, sums, st>>>(a);
   return check_launch("rms_norm_bwd_kernel");
 }
 
@@ -470,12 +585,16 @@ int quantize_for(const void* x, int64_t ldx, int64_t rows, int cols, uint8_t* co
 
 template <typename T>
 int dequantize_for(const uint8_t* codes, const uint8_t* scales, int64_t rows, int cols, void* out, cudaStream_t st) {
-  const bool vec = cols % 8 == 0 && at16(out) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0;
-  const int64_t threads = rows * ceil_div(cols, vec ? 8 : 1);
-  const int64_t want = ceil_div64(threads, 256), most = 16 * static_cast<int64_t>(multiprocessors());
-  const unsigned grid = static_cast<unsigned>(want < most ? want : most);
-  if (vec) mx_dequantize_kernel<T, 8><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
-  else mx_dequantize_kernel<T, 1><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
+  const bool vec = cols % 16 == 0 && at16(out) && at16(codes);
+  const int pieces = ceil_div(cols, vec ? 16 : 1);
+  int bx = 32;
+  while (bx < pieces && bx < 256) bx *= 2;
+  const dim3 block(bx, 256 / bx);
+  const int64_t gx = ceil_div(pieces, bx), want = ceil_div64(rows, 2 * block.y);
+  OMNI_REQUIRE(gx < (int64_t(1) << 31), "too many columns");
+  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(want < 65535 ? want : 65535));
+  if (vec) mx_dequantize_kernel<T, 16><<<grid, block, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
+  else mx_dequantize_kernel<T, 1><<<grid, block, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
   return check_launch("mx_dequantize_kernel");
 }
 
@@ -508,21 +627,22 @@ extern "C" int omni_rms_norm(const void* x, int64_t ldx, const void* residual, i
 
 extern "C" size_t omni_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden) {
   if (rows < 1 || hidden < 1 || hidden > kMaxHidden) return 0;
-  return sizeof(float) * static_cast<size_t>(bwd_blocks(rows, 1)) * hidden;  // a row group each at least
+  const int64_t most = 2 * static_cast<int64_t>(multiprocessors());
+  return sizeof(float) * static_cast<size_t>(rows < most ? rows : most) * hidden;
 }
 
 extern "C" int omni_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, const void* weight,
                                  int w_dtype, int dtype, const float* rstd, int64_t rows, int hidden, void* dx, void* dweight,
-                                 void* scratch, size_t scratch_bytes, void* stream) {
+                                 void* scratch, size_t scratch_bytes, int32_t* status, void* stream) {
   if (int e = check_norm(dtype, w_dtype, rows, hidden)) return e;
   if (rows == 0) return 0;
-  OMNI_REQUIRE(dy && h && weight && rstd && dx, "NULL argument");
+  OMNI_REQUIRE(dy && h && weight && rstd && dx && status, "NULL argument");
   OMNI_REQUIRE(rows == 1 || (lddy >= hidden && ldh >= hidden && (!dh || lddh >= hidden)), "row strides must be at least hidden");
   OMNI_REQUIRE(!dweight || (scratch && scratch_bytes >= omni_rms_norm_bwd_scratch_bytes(rows, hidden)), "the weight's gradient needs %zu bytes of scratch",
                omni_rms_norm_bwd_scratch_bytes(rows, hidden));
   NormBwdArgs a{};
   a.dy = dy, a.dh = dh, a.h = h, a.w = weight, a.lddy = lddy, a.lddh = dh ? lddh : 0, a.ldh = ldh, a.rstd = rstd;
-  a.w_f32 = w_dtype == OMNI_F32, a.T = rows, a.H = hidden, a.dx = dx;
+  a.w_f32 = w_dtype == OMNI_F32, a.T = rows, a.H = hidden, a.dx = dx, a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* s = static_cast<float*>(scratch);
   if (dtype == OMNI_F32) return bwd_for<float>(a, dweight, w_dtype, s, st);

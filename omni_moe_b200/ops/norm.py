@@ -52,7 +52,8 @@ def rms_norm_backward(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Ten
         _lib.check(lib.omni_rms_norm_bwd(
             dy.data_ptr(), dy.stride(0), _lib.ptr(dh), dh.stride(0) if dh is not None else 0, h.data_ptr(), h.stride(0),
             weight.data_ptr(), _lib.dtype_code(weight.dtype), _lib.dtype_code(h.dtype), rstd.data_ptr(), t, n, dx.data_ptr(),
-            _lib.ptr(dw), _lib.ptr(scratch), scratch.numel() if scratch is not None else 0, _lib.stream_ptr(index)))
+            _lib.ptr(dw), _lib.ptr(scratch), scratch.numel() if scratch is not None else 0, _lib.device_status(h.device).data_ptr(),
+            _lib.stream_ptr(index)))
     return dx, dw
 
 

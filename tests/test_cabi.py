@@ -126,7 +126,7 @@ def test_norm_and_mx_rejections(lib):
     assert norm(rows=0)[0] == 0
     assert lib.omni_rms_norm(16, 63, None, 0, 16, 1, 1, 2, 64, 1e-6, 16, None, None, None, None, None) < 0
     assert b"row strides" in lib.omni_last_error()
-    assert lib.omni_rms_norm_bwd(16, 64, None, 0, 16, 64, 16, 1, 1, 16, 2, 64, 16, 16, None, 0, None) < 0
+    assert lib.omni_rms_norm_bwd(16, 64, None, 0, 16, 64, 16, 1, 1, 16, 2, 64, 16, 16, None, 0, 16, None) < 0
     assert b"scratch" in lib.omni_last_error()
     assert lib.omni_mx_quantize(None, 4, 0, 2, 0, None, None, None) < 0 and b"cols" in lib.omni_last_error()
     assert lib.omni_mx_quantize(16, 3, 0, 2, 4, 16, 16, None) < 0 and b"row stride" in lib.omni_last_error()

@@ -189,6 +189,26 @@ def test_strides_alignment_and_dimensions():
         e.y.sum().backward()
 
 
+@pytest.mark.parametrize("n,pad", [(256, 8), (512, 4), (96, 32)])
+def test_many_rows_with_a_stride(n, pad):
+    """The gradient of many rows whose x, dy and dh lie in wider matrices (copied row by row), as of contiguous ones."""
+    from omni_moe_b200.ops import omni_rms_norm_func
+    t = 2500
+    wide = [rand((t, n + pad), torch.bfloat16, k) for k in range(3)]
+    w = rand((n,), torch.bfloat16, 5).requires_grad_()
+
+    def grads(x, dy, dh):
+        x = x.detach().requires_grad_()
+        r = torch.zeros_like(x)
+        out = omni_rms_norm_func(x, w, r)
+        alone = omni_rms_norm_func(x, w)
+        return torch.autograd.grad((out.y, out.h), (x, w), (dy, dh)) + torch.autograd.grad(alone.y, (x, w), dy)
+
+    for a, b in zip(grads(*(v[:, :n] for v in wide)), grads(*(v[:, :n].contiguous() for v in wide))):
+        same = (a.double() - b.double()).abs() <= (2 * half_step(torch.bfloat16) + 1e-4) * b.double().abs() + 1e-5 * float(b.double().abs().max())
+        assert same.all()   # a stride that is no multiple of 16 bytes takes the other kernel: another order of the sums
+
+
 def test_rows_of_zeros_and_not_finite_values():
     from omni_moe_b200.ops import mx_dequantize, omni_rms_norm_func
     x = rand((5, 96), torch.float32, 1)
