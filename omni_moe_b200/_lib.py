@@ -126,6 +126,23 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The torch binding of the short operators (csrc/binding.cpp), which calls the same library.  Raises if it is missing."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _binding as module
+        except ImportError as e:
+            raise RuntimeError(f"the torch binding has not been built or does not load ({e}): run `python -m omni_moe_b200.build`; "
+                               "omni_moe_b200 has no fallback path") from e
+        _binding = module
+    return _binding
+
+
 def check(rc: int) -> None:
     if rc != 0:
         msg = load().omni_last_error().decode()
@@ -142,20 +159,13 @@ def stream_ptr(index: int | None = None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index)
 
 
-class _NoSwitch:
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        pass
-
-
-_NO_SWITCH = _NoSwitch()
-
-
-def on_device(index: int):
-    """Context in which CUDA device ``index`` is current: nothing at all where it is already."""
-    return _NO_SWITCH if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+def status_ptr(t: torch.Tensor) -> int:
+    """Address of the status word of the device that ``t`` is on (see :func:`device_status`)."""
+    index = t.get_device()
+    if index < 0:
+        require_cuda(t)
+    st = _DEVICE_STATUS.get(index)
+    return (st if st is not None else device_status(t.device)).data_ptr()
 
 
 def dtype_code(dt: torch.dtype) -> int:

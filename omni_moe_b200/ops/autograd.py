@@ -213,7 +213,7 @@ def gemm(a: torch.Tensor, b: torch.Tensor, a_transposed: bool = False, b_transpo
     if status is None:
         status = _status(a.device)
     if m and n:
-        with _lib.on_device(a.get_device()):
+        with torch.cuda.device(a.device):
             _lib.check(_lib.load().omni_gemm_bf16(a.data_ptr(), int(a_transposed), a.stride(0), b.data_ptr(), int(b_transposed),
                                                   b.stride(0), m, n, k, out.data_ptr(), out.stride(0), status.data_ptr(),
                                                   _lib.stream_ptr()))

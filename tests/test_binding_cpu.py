@@ -1,0 +1,59 @@
+"""The torch binding of the short operators: it loads, and its errors arrive as Python exceptions.  No GPU."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def binding():
+    from omni_moe_b200 import _lib
+    from omni_moe_b200.build import build
+    build()
+    return _lib.binding()
+
+
+def test_refuses_cpu_tensors(binding):
+    x, w = torch.zeros(4, 64), torch.zeros(64)
+    calls = (lambda: binding.rms_norm(x, w, None, 1e-6, False, 0), lambda: binding.mx_quantize(x),
+             lambda: binding.mx_dequantize(x, x, torch.float32), lambda: binding.decode(*[x] * 8, 4, None, None, 0))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call()
+
+
+def test_public_functions_refuse_cpu_tensors():
+    from omni_moe_b200 import ops
+    x, w = torch.zeros(4, 64), torch.zeros(64)
+    for call in (lambda: ops.omni_rms_norm_func(x, w), lambda: ops.mx_quantize(x), lambda: ops.omni_mlp_ckpt_func(x, x, x, x),
+                 lambda: ops.omni_decode_func(x, x, x, x, x, x, x, x, 4)):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call()
+
+
+def test_argument_types(binding):
+    with pytest.raises(TypeError):
+        binding.rms_norm(torch.zeros(4, 64), None, None, 1e-6, False, 0)
+
+
+def test_linked_against_the_shared_runtime(binding):
+    """A static libstdc++ inside the binding would crash on its first formatted error message."""
+    import os
+    import subprocess
+    out = subprocess.run(["readelf", "-d", os.path.abspath(binding.__file__)], capture_output=True, text=True).stdout
+    assert "libstdc++.so" in out and "libomni_moe_b200.so" in out
+
+
+def test_missing_binding_is_reported(monkeypatch):
+    import builtins
+    from omni_moe_b200 import _lib
+    _lib.load()
+    monkeypatch.setattr(_lib, "_binding", None)
+    real = builtins.__import__
+
+    def without(name, globals=None, locals=None, fromlist=(), level=0):
+        if level and fromlist and "_binding" in fromlist:
+            raise ImportError("not built")
+        return real(name, globals, locals, fromlist, level)
+
+    monkeypatch.setattr(builtins, "__import__", without)
+    with pytest.raises(RuntimeError, match="no fallback"):
+        _lib.binding()
