@@ -1,0 +1,51 @@
+"""RMS norm module and the pre-norm block around the layer.
+
+The reference has the layer alone (omni_moe/modules/omni_moe.py:30-106); this is the half of a decoder block that a model
+puts it into: ``h = hidden + residual``, ``y = layer(norm(h))``, with ``h`` handed on as the next half's residual.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+
+from ..ops.norm import RmsNormOutput, omni_rms_norm_func
+from .omni_moe import OmniMoE, OmniMoEConfig
+
+
+class RMSNorm(nn.Module):
+    """``weight * h / sqrt(mean(h^2) + eps)`` of ``h = x + residual`` over the last dimension
+    (:func:`omni_moe_b200.ops.omni_rms_norm_func`)."""
+
+    def __init__(self, hidden_size: int, eps: float = 1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(hidden_size))
+        self.eps = eps
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, quantize: bool = False) -> RmsNormOutput:
+        return omni_rms_norm_func(x, self.weight, residual, self.eps, quantize)
+
+
+class OmniMoEBlock(nn.Module):
+    """Residual addition, norm and layer: ``(y, h)`` from ``hidden_states`` and the residual stream so far, where ``h`` is the new
+    residual stream and ``y`` what the next block adds to it.
+
+    In eval mode without gradients, up to 64 tokens run as two kernels (norm, :meth:`OmniMoE.decode`); otherwise the layer's
+    :meth:`OmniMoE.forward` follows the norm.  ``checkpoint_bits=8`` keeps the shared MLP's pre-activations in 8 bits for the
+    backward (:meth:`OmniMoE.checkpoint_activations`).
+    """
+
+    DECODE_TOKENS = 64
+
+    def __init__(self, config: OmniMoEConfig, eps: float = 1e-6, checkpoint_bits: int = 16):
+        super().__init__()
+        self.norm = RMSNorm(config.hidden_size, eps)
+        self.layer = OmniMoE(config).checkpoint_activations(checkpoint_bits)
+
+    def forward(self, hidden_states: torch.Tensor, residual: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        out = self.norm(hidden_states, residual)
+        tokens = hidden_states.shape[:-1].numel()
+        if not self.layer.training and not out.y.requires_grad and 0 < tokens <= self.DECODE_TOKENS:
+            return self.layer.decode(out.y), out.h
+        return self.layer(out.y), out.h

@@ -95,7 +95,19 @@ class OmniMoE(nn.Module):
 
         self._buffers_cache: dict = {}
         self._bn_cache = None
+        self._checkpoint_bits = 16
         self.last_routing = None  # (scores, indices, weights) of the latest forward, for inspection
+
+    def checkpoint_activations(self, bits: int = 8) -> "OmniMoE":
+        """What the shared MLP keeps of its gate | up pre-activations for the backward: 16 bits a value (bf16, the default) or
+        8 (MX blocks, :func:`omni_mlp_ckpt_func`): half the memory of the largest saved tensor, at gradients computed from
+        values of 3 mantissa bits.  The output does not change (of a float32 module it does: with 8 bits its MLP is computed
+        on bf16 operands).  The layer's input is kept as it is either way: the router and the routed experts keep the same
+        tensor."""
+        if bits not in (8, 16):
+            raise ValueError(f"activations are kept in 8 or 16 bits, not {bits!r}")
+        self._checkpoint_bits = bits
+        return self
 
     # ------------------------------------------------------------------------------------------
     def _bf16_weight(self, p: torch.Tensor) -> torch.Tensor:
@@ -300,7 +312,7 @@ class OmniMoE(nn.Module):
         operators that run the kernels of this library and carry their own backward.  The router front
         (gates, BatchNorm, log-softmax, selection) is one such operator where its limits allow, otherwise
         torch modules / functions followed by the router op, as in the reference."""
-        from ..ops import omni_expert_func, omni_mlp_func, omni_router_func
+        from ..ops import omni_expert_func, omni_mlp_ckpt_func, omni_mlp_func, omni_router_func
         bsz, seq_len, _ = hidden_states.shape
         x = hidden_states.reshape(-1, self.hidden_size)
         if self._fused_router_front_ok():
@@ -332,7 +344,10 @@ class OmniMoE(nn.Module):
             scores, indices = omni_router_func(log_probs_x, log_probs_y, self.num_expert_sqrt, self.top_k)
         routing_weights = torch.exp(scores)
         experts_states = omni_expert_func(x, self.up_embed.weight, self.down_embed.weight, routing_weights, indices)
-        shared = omni_mlp_func(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight)
+        if getattr(self, "_checkpoint_bits", 16) == 8:
+            shared = omni_mlp_ckpt_func(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, keep_x=True)
+        else:
+            shared = omni_mlp_func(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight)
         self.last_routing = (scores.detach(), indices, routing_weights.detach())
         return (shared + experts_states).view(bsz, seq_len, -1)
 

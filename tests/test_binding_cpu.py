@@ -57,3 +57,12 @@ def test_missing_binding_is_reported(monkeypatch):
     monkeypatch.setattr(builtins, "__import__", without)
     with pytest.raises(RuntimeError, match="no fallback"):
         _lib.binding()
+
+
+def test_block_parameters():
+    from omni_moe_b200.modules import OmniMoEBlock, OmniMoEConfig
+    b = OmniMoEBlock(OmniMoEConfig(64, 128, "silu", 256, 4), eps=1e-5, checkpoint_bits=8)
+    names = set(b.state_dict())
+    assert "norm.weight" in names and "layer.gate_proj.weight" in names and b.norm.weight.shape == (64,) and b.norm.eps == 1e-5
+    with pytest.raises(ValueError, match="8 or 16"):
+        OmniMoEBlock(OmniMoEConfig(64, 128, "silu", 256, 4), checkpoint_bits=32)
