@@ -584,14 +584,17 @@ OMNI_API int omni_mx_dequantize(const void *codes, const void *scales, int64_t r
  * The shared MLP with 8-bit activation checkpoints.  omni_mlp_gate_up_save_mx is omni_mlp_gate_up_limit that keeps the
  * gate | up pre-activations as MX blocks, encoded from the fp32 accumulators in the GEMM's epilogue:
  *   codes [T, 2I] e4m3 (gate in columns [0, I), up in [I, 2I)), scales [T, 2 ceil(I / 32)] e8m0 (the gate's, then the up's)
- * omni_swiglu_bwd_mx is omni_swiglu_bwd_limit on the values they stand for: dgate_up [T, 2I] bf16 and, if act is not
- * NULL, act = silu(gate) * up [T, I] bf16.  limit: 0 = no clamp; the backward decides it on the decoded values.
+ * omni_mlp_dact_swiglu_mx starts the backward on the values they stand for, in the epilogue of one GEMM: with
+ * dact = dy [T, H] @ down_w [H, I] (fp32, never written),
+ *   dgate_up [T, 2I] bf16 = (dact * up * silu'(gate) | dact * silu(gate)) and, if act is not NULL, act = silu(gate) * up [T, I]
+ * limit: 0 = no clamp; the backward decides it on the decoded values.
  */
 OMNI_API int omni_mlp_gate_up_save_mx(const void *x, const void *gate_w, const void *up_w, int64_t num_tokens, int hidden,
                                       int intermediate, float limit, void *act, void *codes, void *scales,
                                       int32_t *status, void *stream);
-OMNI_API int omni_swiglu_bwd_mx(const void *codes, const void *scales, const void *dact, int64_t num_tokens,
-                                int intermediate, float limit, void *dgate_up, void *act, void *stream);
+OMNI_API int omni_mlp_dact_swiglu_mx(const void *dy, const void *down_w, int64_t num_tokens, int hidden, int intermediate,
+                                     const void *codes, const void *scales, float limit, void *dgate_up, void *act,
+                                     int32_t *status, void *stream);
 
 #ifdef __cplusplus
 }

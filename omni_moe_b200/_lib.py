@@ -100,7 +100,8 @@ SIGNATURES = {
     "omni_mx_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
     "omni_mlp_gate_up_save_mx": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p]),
-    "omni_swiglu_bwd_mx": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p]),
+    "omni_mlp_dact_swiglu_mx": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
+                                        c_void_p, c_void_p]),
     "omni_decode_max_tokens": (c_int, []),
     "omni_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "omni_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -228,11 +228,8 @@ variable_list mlp_ckpt_backward(const Tensor& dy, const OptTensor& x, const Tens
   const Tensor dgu = at::empty({t, 2 * i}, bf);
   Tensor act;
   if (need_down) act = at::empty({t, i}, bf);
-  {
-    const Tensor dact = gemm(dy, false, wd, true, status);  // dy [T,H] @ Wd [H,I]
-    check(omni_swiglu_bwd_mx(codes.data_ptr(), scales.data_ptr(), dact.data_ptr(), t, static_cast<int>(i), static_cast<float>(limit),
-                             dgu.data_ptr(), ptr(act), stream_of(dy)));
-  }
+  check(omni_mlp_dact_swiglu_mx(dy.data_ptr(), wd.data_ptr(), t, static_cast<int>(h), static_cast<int>(i), codes.data_ptr(), scales.data_ptr(),
+                                static_cast<float>(limit), dgu.data_ptr(), ptr(act), status_ptr(status), stream_of(dy)));
   // order: the product that reads act right after the kernel that wrote it, the two that read (dgate | dup) back to back
   if (need_down) g[3] = gemm(dy, true, act, true, status);  // dy^T [H,T] @ act [T,I]
   if (need_x) {

@@ -1,7 +1,7 @@
 // Memory-bound helpers of the MLP backward: a bf16 matrix transpose (the tensor-core GEMMs here take
 // both operands with the contraction dimension contiguous, so weight gradients, which contract over
 // tokens, are fed transposed copies) and the SwiGLU derivative.
-#include "mx.cuh"
+#include "common.cuh"
 
 namespace omni {
 namespace {
@@ -114,50 +114,6 @@ __global__ void __launch_bounds__(256) swiglu_bwd_kernel(const __nv_bfloat16* __
   }
 }
 
-// The same derivative from 8-bit pre-activations: codes [T, 2I] e4m3 and scales [T, 2 ceil(I / 32)] e8m0 of (gate | up),
-// decoded on the way in (4.03 bytes read a value of act instead of 6).  A thread has 8 neighbours of one row.
-__global__ void __launch_bounds__(256) swiglu_bwd_mx_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                            const __nv_bfloat16* __restrict__ dact, int64_t T, int I, float limit,
-                                                            __nv_bfloat16* __restrict__ dgu, __nv_bfloat16* __restrict__ act) {
-  const int per_row = I / 8, blocks = (I + mx::kBlock - 1) / mx::kBlock;
-  const int64_t total = T * per_row;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t t = i / per_row;
-    const int c = static_cast<int>(i - t * per_row) * 8;
-    const uint8_t* cg = codes + t * (2 * static_cast<int64_t>(I)) + c;
-    const uint8_t* sg = scales + t * (2 * static_cast<int64_t>(blocks)) + c / mx::kBlock;
-    const uint2 qg = __ldg(reinterpret_cast<const uint2*>(cg)), qu = __ldg(reinterpret_cast<const uint2*>(cg + I));
-    const float fg = mx::pow2(static_cast<int>(__ldg(sg)) - 127), fu = mx::pow2(static_cast<int>(__ldg(sg + blocks)) - 127);
-    const uint4 dv = ldg128(dact + t * I + c);
-    const uint32_t wg[4] = {qg.x, qg.x >> 16, qg.y, qg.y >> 16}, wu[4] = {qu.x, qu.x >> 16, qu.y, qu.y >> 16};
-    const uint32_t wd[4] = {dv.x, dv.y, dv.z, dv.w};
-    uint32_t og[4], ou[4], oa[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 g = mx::decode2(wg[q]), u = mx::decode2(wu[q]), d = bf16x2_to_float2(wd[q]);
-      const float gg[2] = {g.x * fg, g.y * fg}, uu[2] = {u.x * fu, u.y * fu}, dd[2] = {d.x, d.y};
-      float rg[2], ru[2], ra[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        // the clamp of the forward, decided on the decoded value (a value at the limit passes its gradient)
-        const bool g_in = !(limit > 0.f) || !(fabsf(gg[e]) > limit), u_in = !(limit > 0.f) || !(fabsf(uu[e]) > limit);
-        const float gc = g_in ? gg[e] : copysignf(limit, gg[e]), uc = u_in ? uu[e] : copysignf(limit, uu[e]);
-        const float sig = 1.0f / (1.0f + __expf(-gc));
-        const float sl = gc * sig;
-        ra[e] = sl * uc;
-        rg[e] = g_in ? dd[e] * uc * (sig * (1.0f + gc * (1.0f - sig))) : 0.f;
-        ru[e] = u_in ? dd[e] * sl : 0.f;
-      }
-      og[q] = float2_to_bf16x2(rg[0], rg[1]);
-      ou[q] = float2_to_bf16x2(ru[0], ru[1]);
-      oa[q] = float2_to_bf16x2(ra[0], ra[1]);
-    }
-    *reinterpret_cast<uint4*>(dgu + t * 2 * I + c) = make_uint4(og[0], og[1], og[2], og[3]);
-    *reinterpret_cast<uint4*>(dgu + t * 2 * I + I + c) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
-    if (act) *reinterpret_cast<uint4*>(act + t * I + c) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
-  }
-}
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
@@ -199,21 +155,6 @@ extern "C" int omni_swiglu_bwd_limit(const void* gate_up, const void* dact, int6
       static_cast<__nv_bfloat16*>(dgate_up), static_cast<uint16_t*>(dgate_up_t), static_cast<uint16_t*>(act_t), ld_t,
       static_cast<__nv_bfloat16*>(act));
   return check_launch("swiglu_bwd_kernel");
-}
-
-extern "C" int omni_swiglu_bwd_mx(const void* codes, const void* scales, const void* dact, int64_t num_tokens, int intermediate,
-                                  float limit, void* dgate_up, void* act, void* stream) {
-  OMNI_REQUIRE(limit >= 0.f, "limit must be >= 0 (0 = no clamp)");
-  OMNI_REQUIRE(num_tokens >= 0 && intermediate >= 8 && intermediate % 8 == 0, "intermediate must be a positive multiple of 8");
-  if (num_tokens == 0) return 0;
-  OMNI_REQUIRE(codes && scales && dact && dgate_up, "NULL argument");
-  OMNI_REQUIRE(aligned16(codes) && aligned16(dact) && aligned16(dgate_up) && aligned16(act), "pointers must be 16-byte aligned");
-  const int64_t blocks = ceil_div64(num_tokens * (intermediate / 8), 256);
-  OMNI_REQUIRE(blocks < (int64_t(1) << 31), "too many tokens for one launch");
-  swiglu_bwd_mx_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<const __nv_bfloat16*>(dact), num_tokens,
-      intermediate, limit, static_cast<__nv_bfloat16*>(dgate_up), static_cast<__nv_bfloat16*>(act));
-  return check_launch("swiglu_bwd_mx_kernel");
 }
 
 extern "C" int omni_swiglu_bwd(const void* gate_up, const void* dact, int64_t num_tokens, int intermediate, void* dgate_up,

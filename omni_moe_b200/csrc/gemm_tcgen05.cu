@@ -35,12 +35,16 @@ using namespace tc;
 constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, each draining half of the columns
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 
-enum { EPI_F32 = 0, EPI_SWIGLU = 1, EPI_RES = 2, EPI_SWIGLU_CLAMP = 3, EPI_SWIGLU_MX = 4, EPI_SWIGLU_CLAMP_MX = 5 };
+enum { EPI_F32 = 0, EPI_SWIGLU = 1, EPI_RES = 2, EPI_SWIGLU_CLAMP = 3, EPI_SWIGLU_MX = 4, EPI_SWIGLU_CLAMP_MX = 5,
+       EPI_DSWIGLU_MX = 6, EPI_DSWIGLU_CLAMP_MX = 7 };
 // EPI_SWIGLU_CLAMP is EPI_SWIGLU with gate and up limited to [-limit, limit] before the activation; a
 // separate instantiation, so the kernels of the common no-clamp case are compiled without it.
 // The _MX forms also keep the gate | up pre-activations as MX blocks for the backward (pair kernel only).
 __host__ __device__ constexpr bool is_mx(int epi) { return epi == EPI_SWIGLU_MX || epi == EPI_SWIGLU_CLAMP_MX; }
-__host__ __device__ constexpr bool is_clamp(int epi) { return epi == EPI_SWIGLU_CLAMP || epi == EPI_SWIGLU_CLAMP_MX; }
+// EPI_DSWIGLU_MX: the accumulators are the gradient of the activation (dy Wd); the epilogue decodes the checkpoints and writes
+// dgate | dup and, if asked for, the activation itself (pair kernel only).
+__host__ __device__ constexpr bool is_dswiglu(int epi) { return epi == EPI_DSWIGLU_MX || epi == EPI_DSWIGLU_CLAMP_MX; }
+__host__ __device__ constexpr bool is_clamp(int epi) { return epi == EPI_SWIGLU_CLAMP || epi == EPI_SWIGLU_CLAMP_MX || epi == EPI_DSWIGLU_CLAMP_MX; }
 __host__ __device__ constexpr bool is_swiglu(int epi) { return epi == EPI_SWIGLU || epi == EPI_SWIGLU_CLAMP || is_mx(epi); }
 
 struct GemmArgs {
@@ -55,9 +59,11 @@ struct GemmArgs {
   int64_t ldr;
   int tma_out;            // pair kernel: 1 = bf16 output tiles leave through shared memory and TMA stores
   int tma_logits;         // pair kernel: 1 = the fp32 router logits do too (tensor map tm_lg)
-  void* gu_out;           // EPI_SWIGLU: if set, [M, 2N] bf16 that also receives the gate | up pre-activations
+  void* gu_out;           // EPI_SWIGLU: if set, [M, 2N] bf16 that also receives the gate | up pre-activations;
+                          // EPI_DSWIGLU: [M, 2N] bf16 dgate | dup
+  void* act_out;          // EPI_DSWIGLU: if set, [M, N] bf16 silu(gate) * up of the decoded values
   int64_t ldgu;
-  uint8_t* mx_codes;      // _MX: [M, 2N] e4m3 codes of the gate | up pre-activations
+  uint8_t* mx_codes;      // _MX: [M, 2N] e4m3 codes of the gate | up pre-activations (written; read by EPI_DSWIGLU)
   uint8_t* mx_scales;     // _MX: [M, 2 ceil(N / 32)] e8m0 scales (the gate's blocks, then the up's)
   // router tile columns of the fused gate/up + router-gate launch (pair kernel, EPI_SWIGLU only)
   int router_tiles;       // tile columns holding router sub-keys (0 = none); they come first in tile order
@@ -156,13 +162,26 @@ __device__ __forceinline__ void swiglu_chunk(const uint32_t (&ra)[32], const uin
 __device__ __forceinline__ void save_mx_block(const uint32_t (&r)[32], uint8_t* codes, uint8_t* scale, int col0, int col_lim, bool wide) {
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) top = fmaxf(top, mx::finite_abs(__uint_as_float(r[i])));
-  const int s = mx::exponent_of(top);
-  const float inv = mx::pow2(-s);
+  for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(__uint_as_float(r[i])));  // passes over NaN
+  int s;
   uint32_t p[8];
+  if (top <= 3.402823466e38f) {
+    // no infinity: the scaled values can be converted as they are (NaN becomes the NaN code)
+    s = mx::exponent_of(top);
+    const float inv = mx::pow2(-s);
 #pragma unroll
-  for (int q = 0; q < 8; ++q)
-    p[q] = mx::encode4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]), inv);
+    for (int q = 0; q < 8; ++q)
+      p[q] = mx::encode_finite4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]), inv);
+  } else {
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, mx::finite_abs(__uint_as_float(r[i])));
+    s = mx::exponent_of(top);
+    const float inv = mx::pow2(-s);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      p[q] = mx::encode4(__uint_as_float(r[4 * q]), __uint_as_float(r[4 * q + 1]), __uint_as_float(r[4 * q + 2]), __uint_as_float(r[4 * q + 3]), inv);
+  }
   if (wide) {
     st256(codes, p);
   } else {
@@ -179,6 +198,99 @@ __device__ __forceinline__ void save_mx_chunk(const uint32_t (&ra)[32], const ui
   const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.mx_codes) & 31) == 0;
   save_mx_block(ra, c, s, col0, col_lim, wide);
   save_mx_block(rb, c + g.N, s + blocks, col0, col_lim, wide);
+}
+
+// Checkpoints of 32 columns of one row: codes of gate and up and their scales.
+struct MxChunk {
+  uint32_t g[8], u[8];
+  uint32_t sg, su;
+};
+__device__ __forceinline__ void load_mx_chunk(MxChunk& c, const GemmArgs& g, int row, int col0) {
+  if (row >= g.M || col0 >= g.N) return;
+  const uint8_t* p = g.mx_codes + static_cast<int64_t>(row) * (2 * g.N) + col0;
+  const int blocks = (g.N + mx::kBlock - 1) / mx::kBlock;
+  const uint8_t* s = g.mx_scales + static_cast<int64_t>(row) * (2 * blocks) + col0 / mx::kBlock;
+  c.sg = __ldg(s), c.su = __ldg(s + blocks);
+  if (g.N % 16 == 0) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (col0 + 16 * q < g.N) {
+        const uint4 a = ldg128(p + 16 * q), b = ldg128(p + g.N + 16 * q);
+        c.g[4 * q] = a.x, c.g[4 * q + 1] = a.y, c.g[4 * q + 2] = a.z, c.g[4 * q + 3] = a.w;
+        c.u[4 * q] = b.x, c.u[4 * q + 1] = b.y, c.u[4 * q + 2] = b.z, c.u[4 * q + 3] = b.w;
+      }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (col0 + 8 * q < g.N) {
+        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p + 8 * q)), b = __ldg(reinterpret_cast<const uint2*>(p + g.N + 8 * q));
+        c.g[2 * q] = a.x, c.g[2 * q + 1] = a.y, c.u[2 * q] = b.x, c.u[2 * q + 1] = b.y;
+      }
+  }
+}
+
+// Epilogue of the activation's gradient: per value d (fp32 accumulator) and decoded g, u:
+//   act = silu(g) u      dgate = d u silu'(g)      dup = d silu(g)
+// so the gradient of the activation is never rounded nor written.  A lane owns a row; the checkpoints of the next 32
+// columns are on their way while the current ones are worked on, those of the first came before the accumulators.
+template <int EPI, int NCH>
+__device__ __forceinline__ void store_tile_dswiglu(uint32_t taddr, int row, int col_tile, int c_begin, const GemmArgs& g, MxChunk cur) {
+  uint32_t ra[32];
+  tmem_ld32_async(taddr + c_begin, ra);
+  const bool wide = g.N % 16 == 0 && (reinterpret_cast<uintptr_t>(g.gu_out) & 31) == 0 && (reinterpret_cast<uintptr_t>(g.act_out) & 31) == 0;
+#pragma unroll
+  for (int ch = 0; ch < NCH; ++ch) {
+    const int c = c_begin + 32 * ch, col0 = col_tile + c;
+    MxChunk nxt;
+    if (ch + 1 < NCH) load_mx_chunk(nxt, g, row, col0 + 32);
+    float d[32];
+    tmem_ld_wait(ra);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) d[i] = __uint_as_float(ra[i]);
+    if (ch + 1 < NCH) tmem_ld32_async(taddr + c + 32, ra);
+    if (row < g.M && col0 < g.N) {
+      const float fg = mx::pow2(static_cast<int>(cur.sg) - 127), fu = mx::pow2(static_cast<int>(cur.su) - 127);
+      __nv_bfloat16* og = reinterpret_cast<__nv_bfloat16*>(g.gu_out) + static_cast<int64_t>(row) * (2 * g.N) + col0;
+      __nv_bfloat16* oa = reinterpret_cast<__nv_bfloat16*>(g.act_out) + static_cast<int64_t>(row) * g.N + col0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // 16 columns
+        uint32_t pg[8], pu[8], pa[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int i = 16 * h + 2 * q;
+          const float2 gq = mx::decode2(cur.g[i >> 2] >> (8 * (i & 3))), uq = mx::decode2(cur.u[i >> 2] >> (8 * (i & 3)));
+          float vg[2] = {gq.x * fg, gq.y * fg}, vu[2] = {uq.x * fu, uq.y * fu}, rg[2], ru[2], rr[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            // the clamp of the forward, decided on the decoded value (a value at the limit passes its gradient)
+            const bool gi = !is_clamp(EPI) || !(fabsf(vg[e]) > g.limit), ui = !is_clamp(EPI) || !(fabsf(vu[e]) > g.limit);
+            const float gc = gi ? vg[e] : copysignf(g.limit, vg[e]), uc = ui ? vu[e] : copysignf(g.limit, vu[e]);
+            const float sig = __fdividef(1.0f, 1.0f + __expf(-gc));
+            const float sl = gc * sig, dd = d[i + e];
+            rr[e] = sl * uc;
+            rg[e] = gi ? dd * uc * __fmaf_rn(sl, 1.0f - sig, sig) : 0.f;
+            ru[e] = ui ? dd * sl : 0.f;
+          }
+          pg[q] = float2_to_bf16x2(rg[0], rg[1]), pu[q] = float2_to_bf16x2(ru[0], ru[1]), pa[q] = float2_to_bf16x2(rr[0], rr[1]);
+        }
+        if (wide) {
+          if (col0 + 16 * h < g.N) {
+            st256(og + 16 * h, pg), st256(og + g.N + 16 * h, pu);
+            if (g.act_out) st256(oa + 16 * h, pa);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (col0 + 16 * h + 8 * q < g.N) {
+              *reinterpret_cast<uint4*>(og + 16 * h + 8 * q) = make_uint4(pg[4 * q], pg[4 * q + 1], pg[4 * q + 2], pg[4 * q + 3]);
+              *reinterpret_cast<uint4*>(og + g.N + 16 * h + 8 * q) = make_uint4(pu[4 * q], pu[4 * q + 1], pu[4 * q + 2], pu[4 * q + 3]);
+              if (g.act_out) *reinterpret_cast<uint4*>(oa + 16 * h + 8 * q) = make_uint4(pa[4 * q], pa[4 * q + 1], pa[4 * q + 2], pa[4 * q + 3]);
+            }
+        }
+      }
+    }
+    cur = nxt;
+  }
 }
 
 // Drains this warp's share of one accumulator tile: its 32 rows (TMEM lane quarter) and the column
@@ -828,13 +940,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int tn = router_tile ? tn_all : tn_all - rt;
       const int acc = it & 1;
       const uint32_t acc_phase = (it >> 1) & 1;
+      const int row = tm * (2 * BM) + static_cast<int>(rank) * BM + quarter * 32 + lane;
+      constexpr int OUTC = (is_swiglu(EPI)) ? BN / 2 : BN;
+      MxChunk mx_first;
+      if constexpr (is_dswiglu(EPI)) load_mx_chunk(mx_first, g, row, tn * OUTC + col_half * (OUTC / 2));
       bool ok;
       OMNI_TIMED(e_wait, ok = mbar_wait(bar_tfull + 8 * acc, acc_phase, abort_flag, g.status));
       tc_fence_after();
       if (!ok) break;
-      const int row = tm * (2 * BM) + static_cast<int>(rank) * BM + quarter * 32 + lane;
       const uint32_t taddr = tmem_base + acc * BN + (static_cast<uint32_t>(quarter * 32) << 16);
-      constexpr int OUTC = (is_swiglu(EPI)) ? BN / 2 : BN;
       if (router_tile) {
         // accumulator columns [0, 128) are x-axis sub-keys tn*128.., [128, 256) the y-axis ones;
         // the warps of column half h store axis h
@@ -846,6 +960,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                               bars + 1024 + static_cast<uint32_t>(warp - 2) * 4096);
         else
           store_tile<BN, EPI_F32, 4>(taddr + col_half * (BN / 2), row, col_tile, (col_half + 1) * g.router_n, 0, gr);
+      } else if constexpr (is_dswiglu(EPI)) {
+        OMNI_TIMED(e_store, (store_tile_dswiglu<EPI, OUTC / 64>(taddr, row, tn * OUTC, col_half * (OUTC / 2), g, mx_first)));
       } else if (g.tma_out) {
         const uint32_t stg = bars + 1024 + static_cast<uint32_t>(warp - 2) * 4096;
         OMNI_TIMED(e_store, (store_tile_tma<BN, EPI, OUTC / 64>(taddr, row - lane, tn * OUTC, g.N, col_half * (OUTC / 2), g, &tm_out, stg)));
@@ -1319,6 +1435,30 @@ extern "C" int omni_gemm_bf16_stacked_b(const void* a, int a_transposed, int64_t
                static_cast<long long>(k_split));
   OMNI_REQUIRE(aligned16(b1), "pointers must be 16-byte aligned");
   return gemm_bf16_impl(a, a_transposed, lda, b0, b1, k_split, 1, ldb, m, n, k, out, ldo, status, stream);
+}
+
+extern "C" int omni_mlp_dact_swiglu_mx(const void* dy, const void* down_w, int64_t num_tokens, int hidden, int intermediate,
+                                       const void* codes, const void* scales, float limit, void* dgate_up, void* act, int32_t* status,
+                                       void* stream) {
+  OMNI_REQUIRE(num_tokens >= 0 && num_tokens < (int64_t(1) << 31) - 2 * BM, "num_tokens out of range");
+  OMNI_REQUIRE(hidden >= 8 && hidden % 8 == 0, "hidden must be a positive multiple of 8, got %d", hidden);
+  OMNI_REQUIRE(intermediate >= 8 && intermediate % 8 == 0, "intermediate must be a positive multiple of 8, got %d", intermediate);
+  OMNI_REQUIRE(limit >= 0.f, "limit must be >= 0 (0 = no clamp), got %g", static_cast<double>(limit));  // also refuses NaN
+  if (num_tokens == 0) return 0;
+  OMNI_REQUIRE(dy && down_w && codes && scales && dgate_up && status, "NULL argument");
+  OMNI_REQUIRE(aligned16(dy) && aligned16(down_w) && aligned16(codes) && aligned16(dgate_up) && aligned16(act), "pointers must be 16-byte aligned");
+  CUtensorMap ma, mb;
+  if (int e = make_map(&ma, dy, num_tokens, hidden, BM)) return e;
+  if (int e = make_map(&mb, down_w, hidden, intermediate, 64)) return e;  // [K, N]: boxes of 64 K rows
+  GemmArgs g{};
+  g.M = static_cast<int>(num_tokens), g.N = intermediate, g.K = hidden, g.dual = 0;
+  g.tiles_m = ceil_div(g.M, 2 * BM);
+  g.tiles_n = g.tiles_n_axis = ceil_div(g.N, 256);
+  g.gu_out = dgate_up, g.act_out = act, g.limit = limit, g.status = status;
+  g.mx_codes = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes)), g.mx_scales = const_cast<uint8_t*>(static_cast<const uint8_t*>(scales));
+  OMNI_SET_TUNING(g);
+  if (limit > 0.f) return launch_pair<EPI_DSWIGLU_CLAMP_MX, false, 1>(ma, mb, mb, mb, mb, g, static_cast<cudaStream_t>(stream));
+  return launch_pair<EPI_DSWIGLU_MX, false, 1>(ma, mb, mb, mb, mb, g, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int omni_mlp_fwd(const void* x, const void* gate_w, const void* up_w, const void* down_w, int64_t num_tokens,

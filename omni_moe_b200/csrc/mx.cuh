@@ -40,6 +40,14 @@ __device__ __forceinline__ uint32_t encode4(float v0, float v1, float v2, float 
   return encode2(v0, v1, inv) | (encode2(v2, v3, inv) << 16);
 }
 
+// The same where no value is infinite: NaN converts to the NaN code by itself.
+__device__ __forceinline__ uint32_t encode_finite4(float v0, float v1, float v2, float v3, float inv) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v1 * inv), "f"(v0 * inv));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v3 * inv), "f"(v2 * inv));
+  return lo | (static_cast<uint32_t>(hi) << 16);
+}
+
 // The two e4m3 values in the low 16 bits of r.
 __device__ __forceinline__ float2 decode2(uint32_t r) {
   uint32_t h;

@@ -142,6 +142,11 @@ def test_mlp_checkpoint_rejections(lib):
         rc, msg = save(**kw)
         assert rc < 0 and what in msg, (kw, msg)
     assert save(t=0)[0] == 0
-    assert lib.omni_swiglu_bwd_mx(None, None, None, 4, 12, 0.0, None, None, None) < 0 and b"multiple of 8" in lib.omni_last_error()
-    assert lib.omni_swiglu_bwd_mx(None, None, None, 4, 16, 0.0, None, None, None) < 0 and b"NULL" in lib.omni_last_error()
-    assert lib.omni_swiglu_bwd_mx(None, None, None, 4, 16, -1.0, None, None, None) < 0 and b"limit" in lib.omni_last_error()
+    def dact(t=4, h=64, i=64, limit=0.0):
+        return lib.omni_mlp_dact_swiglu_mx(None, None, t, h, i, None, None, limit, None, None, None, None), lib.omni_last_error()
+
+    for kw, what in ((dict(t=-1), b"num_tokens"), (dict(h=4), b"hidden"), (dict(i=12), b"intermediate"), (dict(limit=-1.0), b"limit"),
+                     (dict(limit=float("nan")), b"limit"), (dict(), b"NULL")):
+        rc, msg = dact(**kw)
+        assert rc < 0 and what in msg, (kw, msg)
+    assert dact(t=0)[0] == 0
