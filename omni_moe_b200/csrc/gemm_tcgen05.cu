@@ -159,7 +159,7 @@ __device__ __forceinline__ void swiglu_chunk(const uint32_t (&ra)[32], const uin
 // block, so its maximum needs no shuffle.  Columns from col_lim on are not stored; their accumulators are zero (the
 // tensor map fills weight rows outside the matrix with zeros) and do not count.  codes: this row's codes at col0; `wide`:
 // the whole block can be stored as one 32-byte sector.
-__device__ __forceinline__ void save_mx_block(const uint32_t (&r)[32], uint8_t* codes, uint8_t* scale, int col0, int col_lim, bool wide) {
+__device__ __forceinline__ uint32_t save_mx_block(const uint32_t (&r)[32], uint8_t* codes, int col0, int col_lim, bool wide) {
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(__uint_as_float(r[i])));  // passes over NaN
@@ -189,29 +189,62 @@ __device__ __forceinline__ void save_mx_block(const uint32_t (&r)[32], uint8_t* 
     for (int q = 0; q < 4; ++q)
       if (col0 + 8 * q < col_lim) *reinterpret_cast<uint2*>(codes + 8 * q) = make_uint2(p[2 * q], p[2 * q + 1]);
   }
-  *scale = static_cast<uint8_t>(s + 127);
+  return static_cast<uint32_t>(s + 127);
 }
-__device__ __forceinline__ void save_mx_chunk(const uint32_t (&ra)[32], const uint32_t (&rb)[32], int row, int col0, int col_lim, const GemmArgs& g) {
+// Chunk `ch` of two; the scales of both go out together with the second (or with the first, where the second lies outside).
+__device__ __forceinline__ void save_mx_chunk(const uint32_t (&ra)[32], const uint32_t (&rb)[32], int row, int col0, int col_lim, const GemmArgs& g,
+                                              int ch, uint32_t& sg, uint32_t& su) {
   uint8_t* c = g.mx_codes + static_cast<int64_t>(row) * (2 * g.N) + col0;
-  const int blocks = (g.N + mx::kBlock - 1) / mx::kBlock;
-  uint8_t* s = g.mx_scales + static_cast<int64_t>(row) * (2 * blocks) + col0 / mx::kBlock;
   const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.mx_codes) & 31) == 0;
-  save_mx_block(ra, c, s, col0, col_lim, wide);
-  save_mx_block(rb, c + g.N, s + blocks, col0, col_lim, wide);
+  const uint32_t vg = save_mx_block(ra, c, col0, col_lim, wide), vu = save_mx_block(rb, c + g.N, col0, col_lim, wide);
+  if ((ch & 1) == 0) sg = vg, su = vu;
+  else sg |= vg << 8, su |= vu << 8;
+  const bool last = col0 + 32 >= col_lim;
+  if ((ch & 1) == 0 && !last) return;
+  const int blocks = (g.N + mx::kBlock - 1) / mx::kBlock;
+  uint8_t* s = g.mx_scales + static_cast<int64_t>(row) * (2 * blocks) + (col0 / mx::kBlock - (ch & 1));
+  if ((ch & 1) && (blocks & 1) == 0 && (reinterpret_cast<uintptr_t>(g.mx_scales) & 1) == 0) {
+    *reinterpret_cast<uint16_t*>(s) = static_cast<uint16_t>(sg), *reinterpret_cast<uint16_t*>(s + blocks) = static_cast<uint16_t>(su);
+  } else {
+    s[0] = static_cast<uint8_t>(sg), s[blocks] = static_cast<uint8_t>(su);
+    if (ch & 1) s[1] = static_cast<uint8_t>(sg >> 8), s[blocks + 1] = static_cast<uint8_t>(su >> 8);
+  }
 }
 
-// Checkpoints of 32 columns of one row: codes of gate and up and their scales.
+// 256-bit read-only load (a whole 32-byte sector); ptr must be 32-byte aligned.
+__device__ __forceinline__ void ld256(const void* ptr, uint32_t (&p)[8]) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3]), "=r"(p[4]), "=r"(p[5]), "=r"(p[6]), "=r"(p[7])
+               : "l"(ptr));
+}
+
+// Checkpoints of 32 columns of one row: codes of gate and up.
 struct MxChunk {
   uint32_t g[8], u[8];
-  uint32_t sg, su;
 };
+// Scales of the four chunks of 32 columns that a warp drains of one row, as bytes of a word.
+struct MxScales {
+  uint32_t g, u;
+};
+__device__ __forceinline__ void load_mx_scales(MxScales& c, const GemmArgs& g, int row, int col0) {
+  c.g = c.u = 0;
+  if (row >= g.M || col0 >= g.N) return;
+  const int blocks = (g.N + mx::kBlock - 1) / mx::kBlock, b0 = col0 / mx::kBlock;
+  const uint8_t* s = g.mx_scales + static_cast<int64_t>(row) * (2 * blocks) + b0;
+  if (blocks % 4 == 0 && (reinterpret_cast<uintptr_t>(g.mx_scales) & 3) == 0) {
+    c.g = __ldg(reinterpret_cast<const uint32_t*>(s)), c.u = __ldg(reinterpret_cast<const uint32_t*>(s + blocks));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (b0 + q < blocks) c.g |= static_cast<uint32_t>(__ldg(s + q)) << (8 * q), c.u |= static_cast<uint32_t>(__ldg(s + blocks + q)) << (8 * q);
+  }
+}
 __device__ __forceinline__ void load_mx_chunk(MxChunk& c, const GemmArgs& g, int row, int col0) {
   if (row >= g.M || col0 >= g.N) return;
   const uint8_t* p = g.mx_codes + static_cast<int64_t>(row) * (2 * g.N) + col0;
-  const int blocks = (g.N + mx::kBlock - 1) / mx::kBlock;
-  const uint8_t* s = g.mx_scales + static_cast<int64_t>(row) * (2 * blocks) + col0 / mx::kBlock;
-  c.sg = __ldg(s), c.su = __ldg(s + blocks);
-  if (g.N % 16 == 0) {
+  if (g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.mx_codes) & 31) == 0) {
+    ld256(p, c.g), ld256(p + g.N, c.u);
+  } else if (g.N % 16 == 0) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
       if (col0 + 16 * q < g.N) {
@@ -234,7 +267,8 @@ __device__ __forceinline__ void load_mx_chunk(MxChunk& c, const GemmArgs& g, int
 // so the gradient of the activation is never rounded nor written.  A lane owns a row; the checkpoints of the next 32
 // columns are on their way while the current ones are worked on, those of the first came before the accumulators.
 template <int EPI, int NCH>
-__device__ __forceinline__ void store_tile_dswiglu(uint32_t taddr, int row, int col_tile, int c_begin, const GemmArgs& g, MxChunk cur) {
+__device__ __forceinline__ void store_tile_dswiglu(uint32_t taddr, int row, int col_tile, int c_begin, const GemmArgs& g, MxChunk cur, const MxScales& scales) {
+  static_assert(NCH == 4, "scales of four chunks");
   uint32_t ra[32];
   tmem_ld32_async(taddr + c_begin, ra);
   const bool wide = g.N % 16 == 0 && (reinterpret_cast<uintptr_t>(g.gu_out) & 31) == 0 && (reinterpret_cast<uintptr_t>(g.act_out) & 31) == 0;
@@ -249,7 +283,7 @@ __device__ __forceinline__ void store_tile_dswiglu(uint32_t taddr, int row, int 
     for (int i = 0; i < 32; ++i) d[i] = __uint_as_float(ra[i]);
     if (ch + 1 < NCH) tmem_ld32_async(taddr + c + 32, ra);
     if (row < g.M && col0 < g.N) {
-      const float fg = mx::pow2(static_cast<int>(cur.sg) - 127), fu = mx::pow2(static_cast<int>(cur.su) - 127);
+      const float fg = mx::pow2(static_cast<int>((scales.g >> (8 * ch)) & 0xff) - 127), fu = mx::pow2(static_cast<int>((scales.u >> (8 * ch)) & 0xff) - 127);
       __nv_bfloat16* og = reinterpret_cast<__nv_bfloat16*>(g.gu_out) + static_cast<int64_t>(row) * (2 * g.N) + col0;
       __nv_bfloat16* oa = reinterpret_cast<__nv_bfloat16*>(g.act_out) + static_cast<int64_t>(row) * g.N + col0;
 #pragma unroll
@@ -265,7 +299,8 @@ __device__ __forceinline__ void store_tile_dswiglu(uint32_t taddr, int row, int 
             // the clamp of the forward, decided on the decoded value (a value at the limit passes its gradient)
             const bool gi = !is_clamp(EPI) || !(fabsf(vg[e]) > g.limit), ui = !is_clamp(EPI) || !(fabsf(vu[e]) > g.limit);
             const float gc = gi ? vg[e] : copysignf(g.limit, vg[e]), uc = ui ? vu[e] : copysignf(g.limit, vu[e]);
-            const float sig = __fdividef(1.0f, 1.0f + __expf(-gc));
+            float sig;
+            asm("rcp.approx.f32 %0, %1;" : "=f"(sig) : "f"(1.0f + __expf(-gc)));
             const float sl = gc * sig, dd = d[i + e];
             rr[e] = sl * uc;
             rg[e] = gi ? dd * uc * __fmaf_rn(sl, 1.0f - sig, sig) : 0.f;
@@ -301,6 +336,7 @@ __device__ __forceinline__ void store_tile_dswiglu(uint32_t taddr, int row, int 
 template <int BN, int EPI, int NCH>
 __device__ __forceinline__ void store_tile(uint32_t taddr, int row, int col_tile, int col_lim, int c_begin, const GemmArgs& g) {
   uint32_t ra[32], rb[32];
+  [[maybe_unused]] uint32_t mx_sg = 0, mx_su = 0;
   tmem_ld32_async(taddr + c_begin, ra);
   if (is_swiglu(EPI)) tmem_ld32_async(taddr + BN / 2 + c_begin, rb);
 #pragma unroll
@@ -326,7 +362,7 @@ __device__ __forceinline__ void store_tile(uint32_t taddr, int row, int col_tile
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ra[i]);
     }
     if constexpr (is_mx(EPI)) {
-      if (live) save_mx_chunk(ra, rb, row, col0, col_lim, g);
+      if (live) save_mx_chunk(ra, rb, row, col0, col_lim, g, ch, mx_sg, mx_su);
     }
     if (is_swiglu(EPI) && !is_mx(EPI) && g.gu_out != nullptr && live) {
       // training: keep the pre-activations for the backward (gate in columns [0, N), up in [N, 2N))
@@ -443,6 +479,7 @@ __device__ __forceinline__ void store_tile_tma(uint32_t taddr, int row0, int col
   const int lane = lane_id();
   const int row = row0 + lane;
   uint32_t ra[32], rb[32];
+  [[maybe_unused]] uint32_t mx_sg = 0, mx_su = 0;
   tmem_ld32_async(taddr + c_begin, ra);
   if (is_swiglu(EPI)) tmem_ld32_async(taddr + BN / 2 + c_begin, rb);
 #pragma unroll
@@ -461,7 +498,7 @@ __device__ __forceinline__ void store_tile_tma(uint32_t taddr, int row0, int col
       for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ra[i]);
     }
     if constexpr (is_mx(EPI)) {
-      if (live) save_mx_chunk(ra, rb, row, col0, col_lim, g);
+      if (live) save_mx_chunk(ra, rb, row, col0, col_lim, g, ch, mx_sg, mx_su);
     }
     if (is_swiglu(EPI) && !is_mx(EPI) && g.gu_out != nullptr && live) {
       __nv_bfloat16* og = reinterpret_cast<__nv_bfloat16*>(g.gu_out) + static_cast<int64_t>(row) * g.ldgu + col0;
@@ -943,7 +980,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int row = tm * (2 * BM) + static_cast<int>(rank) * BM + quarter * 32 + lane;
       constexpr int OUTC = (is_swiglu(EPI)) ? BN / 2 : BN;
       MxChunk mx_first;
-      if constexpr (is_dswiglu(EPI)) load_mx_chunk(mx_first, g, row, tn * OUTC + col_half * (OUTC / 2));
+      MxScales mx_scales;
+      if constexpr (is_dswiglu(EPI)) {
+        load_mx_scales(mx_scales, g, row, tn * OUTC + col_half * (OUTC / 2));
+        load_mx_chunk(mx_first, g, row, tn * OUTC + col_half * (OUTC / 2));
+      }
       bool ok;
       OMNI_TIMED(e_wait, ok = mbar_wait(bar_tfull + 8 * acc, acc_phase, abort_flag, g.status));
       tc_fence_after();
@@ -961,7 +1002,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         else
           store_tile<BN, EPI_F32, 4>(taddr + col_half * (BN / 2), row, col_tile, (col_half + 1) * g.router_n, 0, gr);
       } else if constexpr (is_dswiglu(EPI)) {
-        OMNI_TIMED(e_store, (store_tile_dswiglu<EPI, OUTC / 64>(taddr, row, tn * OUTC, col_half * (OUTC / 2), g, mx_first)));
+        OMNI_TIMED(e_store, (store_tile_dswiglu<EPI, OUTC / 64>(taddr, row, tn * OUTC, col_half * (OUTC / 2), g, mx_first, mx_scales)));
       } else if (g.tma_out) {
         const uint32_t stg = bars + 1024 + static_cast<uint32_t>(warp - 2) * 4096;
         OMNI_TIMED(e_store, (store_tile_tma<BN, EPI, OUTC / 64>(taddr, row - lane, tn * OUTC, g.N, col_half * (OUTC / 2), g, &tm_out, stg)));
