@@ -12,6 +12,8 @@
 // Gradient of the weight: a block walks over rows with a stride of the grid and keeps the sums of its columns in
 // registers; one partial row per block goes to scratch and a second kernel adds the partial rows in block order (no
 // atomics: run-to-run identical).
+#include <type_traits>
+
 #include "mx.cuh"
 #include "tcgen05.cuh"
 
@@ -19,7 +21,6 @@ namespace omni {
 namespace {
 
 constexpr int kMaxHidden = 16384;
-constexpr int kPerThread = 32;  // values of a row in one thread
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -41,7 +42,7 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 // VE neighbouring values moved by one instruction: 16 bytes, or a single value where a row's address or length does
 // not allow more.
 template <typename T, int VE>
-struct Pack {
+struct __align__(sizeof(T) * VE < 16 ? sizeof(T) * VE : 16) Pack {
   T v[VE];
 };
 template <typename T, int VE>
@@ -66,6 +67,45 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, VE>& r) {
   } else *p = r.v[0];
 }
 
+// Pieces to fp32 and back, two 16-bit values at a time: a bf16 is the upper half of an fp32, so unpacking is a shift and a
+// mask, and one conversion packs two.  (Value by value the compiler spends a register and two instructions on each half.)
+template <typename T, int VE>
+__device__ __forceinline__ void unpack(const Pack<T, VE>& p, float (&f)[VE]) {
+  if constexpr (sizeof(T) == 2 && VE % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+#pragma unroll
+    for (int i = 0; i < VE / 2; ++i) {
+      float2 v;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) v = bf16x2_to_float2(w[i]);
+      else v = __half22float2(*reinterpret_cast<const __half2*>(w + i));
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = to_f<T>(p.v[e]);
+  }
+}
+template <typename T, int VE>
+__device__ __forceinline__ Pack<T, VE> pack(const float (&f)[VE]) {
+  Pack<T, VE> p;
+  if constexpr (sizeof(T) == 2 && VE % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+    for (int i = 0; i < VE / 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        w[i] = float2_to_bf16x2(f[2 * i], f[2 * i + 1]);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) p.v[e] = from_f<T>(f[e]);
+  }
+  return p;
+}
+
 // w[c .. c + VE) as fp32, from a vector of the data's type or of fp32.
 template <typename T, int VE>
 __device__ __forceinline__ void load_weight(const void* w, bool w_f32, int c, float (&out)[VE]) {
@@ -81,9 +121,7 @@ __device__ __forceinline__ void load_weight(const void* w, bool w_f32, int c, fl
       out[0] = __ldg(static_cast<const float*>(w) + c);
     }
   } else {
-    const Pack<T, VE> p = load_pack<T, VE>(static_cast<const T*>(w) + c);
-#pragma unroll
-    for (int e = 0; e < VE; ++e) out[e] = to_f<T>(p.v[e]);
+    unpack<T, VE>(load_pack<T, VE>(static_cast<const T*>(w) + c), out);
   }
 }
 
@@ -99,14 +137,22 @@ __device__ __forceinline__ float row_sum(float v, int warps, int grp, int warp_i
   return s;
 }
 
-// The MX codes of this thread's VE values of one pack (all lanes of the block's group call this; dead lanes pass zeros).
+// The scale's exponent of the MX block that this thread's VE values belong to.  All lanes of the warp call this; dead lanes
+// pass zeros.  The maximum passes over NaN; an infinity in it sends the warp to the careful form.
 template <int VE>
 __device__ __forceinline__ int block_exponent(const float (&y)[VE]) {
   float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) top = fmaxf(top, mx::finite_abs(y[e]));
+  for (int e = 0; e < VE; ++e) top = fmaxf(top, fabsf(y[e]));
 #pragma unroll
   for (int o = 1; o < mx::kBlock / VE; o <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+  if (__any_sync(FULL_MASK, top > 3.402823466e38f)) {
+    top = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) top = fmaxf(top, mx::finite_abs(y[e]));
+#pragma unroll
+    for (int o = 1; o < mx::kBlock / VE; o <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+  }
   return mx::exponent_of(top);
 }
 template <int VE>
@@ -158,16 +204,19 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
   for (int i = 0; i < V; ++i) {
     const int c = (i * tpr + tid) * VE;
     if (live && c < a.H) {
+      float f[VE];
+      unpack<T, VE>(px[i], f);
       if (a.r) {
+        float q[VE];
+        unpack<T, VE>(pr[i], q);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) px[i].v[e] = from_f<T>(to_f<T>(px[i].v[e]) + to_f<T>(pr[i].v[e]));
+        for (int e = 0; e < VE; ++e) f[e] += q[e];
+        px[i] = pack<T, VE>(f);
         store_pack<T, VE>(static_cast<T*>(a.h) + t * a.H + c, px[i]);
+        unpack<T, VE>(px[i], f);
       }
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float f = to_f<T>(px[i].v[e]);
-        sq = __fmaf_rn(f, f * a.shrink, sq);
-      }
+      for (int e = 0; e < VE; ++e) sq = __fmaf_rn(f[e], f[e] * a.shrink, sq);
     }
   }
   sq = row_sum(sq, a.warps, grp, tid >> 5, s_sum);
@@ -184,13 +233,10 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
     if (in) {
       float w[VE];
       load_weight<T, VE>(a.w, a.w_f32, c, w);
-      Pack<T, VE> o;
+      unpack<T, VE>(px[i], y);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        y[e] = to_f<T>(px[i].v[e]) * rho * w[e];
-        o.v[e] = from_f<T>(y[e]);
-      }
-      store_pack<T, VE>(static_cast<T*>(a.y) + t * a.H + c, o);
+      for (int e = 0; e < VE; ++e) y[e] = y[e] * rho * w[e];
+      store_pack<T, VE>(static_cast<T*>(a.y) + t * a.H + c, pack<T, VE>(y));
     }
     if (a.codes) {
       const int s = block_exponent<VE>(y);
@@ -209,6 +255,7 @@ struct NormBwdArgs {
   int w_f32;
   int64_t T;
   int H;
+  float per_value;  // 1 / H
   int warps, rpc;
   void* dx;
   float* partial;  // [blocks, H] or null
@@ -243,32 +290,34 @@ __device__ __forceinline__ void bwd_row(const NormBwdArgs& a, const Pack<T, VE> 
   for (int i = 0; i < V; ++i) {
     const int c = (i * tpr + tid) * VE;
     if (live && c < a.H) {
-      float w[VE];
+      float w[VE], h[VE], g[VE];
       load_weight<T, VE>(a.w, a.w_f32, c, w);
+      unpack<T, VE>(ph[i], h), unpack<T, VE>(pg[i], g);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float g = to_f<T>(pg[i].v[e]), n = to_f<T>(ph[i].v[e]) * rho;
-        dw[i][e] = __fmaf_rn(g, n, dw[i][e]);
-        dot = __fmaf_rn(g * w[e], n, dot);
+        const float n = h[e] * rho;
+        dw[i][e] = __fmaf_rn(g[e], n, dw[i][e]);
+        dot = __fmaf_rn(g[e] * w[e], n, dot);
       }
     }
   }
-  dot = row_sum(dot, a.warps, grp, tid >> 5, s_sum) / static_cast<float>(a.H);
+  dot = row_sum(dot, a.warps, grp, tid >> 5, s_sum) * a.per_value;
+  const float back = -dot * rho * rho;  // rho (dz - h rho dot) = rho dz + h (-dot rho^2)
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = (i * tpr + tid) * VE;
     if (live && c < a.H) {
-      float w[VE];
+      float w[VE], h[VE], g[VE];
       load_weight<T, VE>(a.w, a.w_f32, c, w);
-      Pack<T, VE> o;
+      unpack<T, VE>(ph[i], h), unpack<T, VE>(pg[i], g);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float n = to_f<T>(ph[i].v[e]) * rho;
-        float d = rho * __fmaf_rn(-n, dot, to_f<T>(pg[i].v[e]) * w[e]);
-        if (a.dh) d += to_f<T>(pd[i].v[e]);
-        o.v[e] = from_f<T>(d);
+      for (int e = 0; e < VE; ++e) g[e] = __fmaf_rn(h[e], back, rho * (g[e] * w[e]));
+      if (a.dh) {
+        unpack<T, VE>(pd[i], h);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) g[e] += h[e];
       }
-      store_pack<T, VE>(static_cast<T*>(a.dx) + t * a.H + c, o);
+      store_pack<T, VE>(static_cast<T*>(a.dx) + t * a.H + c, pack<T, VE>(g));
     }
   }
 }
@@ -308,9 +357,10 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const NormBwdArgs a) 
 }
 
 // Many rows: the copy engine brings whole rows into a ring of shared-memory stages (rpc rows of h, dy and dh each), ahead
-// of the threads, so that the barrier of a row's sum leaves no gap in the traffic.  (16384 x 4096 bf16: rows into registers
-// 191 us, the next row's registers loaded ahead 140 us.)
-constexpr int kBwdStages = 3;
+// of the threads, so that the barrier of a row's sum leaves no gap in the traffic.  (16384 x 4096 bf16 with dh: rows into
+// registers 191 us, the next row's registers loaded ahead 140, ring 124, with two stages and a third block on the
+// multiprocessor 97 = 5.5 TB/s; a producer warp of its own for the copies gains nothing.)
+constexpr int kBwdStages = 2;
 template <typename T, int VE, int V>
 __global__ void __launch_bounds__(512) rms_norm_bwd_ring_kernel(const NormBwdArgs a) {
   __shared__ float s_sum[2 * 8 * 16];
@@ -381,22 +431,23 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_ring_kernel(const NormBwdArg
   if (a.partial) put_partial<VE, V>(a, dw, reinterpret_cast<float*>(s_dyn), tpr, grp, tid);
 }
 
-// dw[c] = the sum of the partial rows in block order: 32 columns x 8 slices of rows a block.
-__global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ partial, int blocks, int H, void* dw, int dtype) {
-  __shared__ float s_part[8][32];
+// dw[c] = the sum of the partial rows in block order: 32 columns x 32 slices of rows a block.
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float* __restrict__ partial, int blocks, int H, void* dw, int dtype) {
+  __shared__ float s_part[32][33];
   const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + col;
   float s = 0.f;
   if (c < H) {
-#pragma unroll 8
-    for (int b = slice; b < blocks; b += 8) s += partial[static_cast<int64_t>(b) * H + c];
+#pragma unroll 4
+    for (int b = slice; b < blocks; b += 32) s += partial[static_cast<int64_t>(b) * H + c];
   }
   s_part[slice][col] = s;
   __syncthreads();
-  if (slice == 0 && c < H) {
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v += s_part[i][col];
+  // warp w adds the 32 slices of column w, one in each lane
+  const float v = warp_sum(s_part[col][slice]);
+  const int wc = blockIdx.x * 32 + slice;
+  if (col == 0 && wc < H) {
+    const int c = wc;
     if (dtype == OMNI_F32) static_cast<float*>(dw)[c] = v;
     else if (dtype == OMNI_BF16) static_cast<__nv_bfloat16*>(dw)[c] = __float2bfloat16_rn(v);
     else static_cast<__half*>(dw)[c] = __float2half_rn(v);
@@ -449,6 +500,22 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
     if constexpr (VE == 16) {
       const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
       const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+      if constexpr (sizeof(T) == 2) {
+        if ((reinterpret_cast<uintptr_t>(out) & 31) == 0) {  // 32 bytes in one store (two halves of a sector: 39 us instead)
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f0 = mx::decode2(w[e]), f1 = mx::decode2(w[e] >> 16);
+            Pack<T, 4> v;
+            v.v[0] = from_f<T>(f0.x * sc), v.v[1] = from_f<T>(f0.y * sc), v.v[2] = from_f<T>(f1.x * sc), v.v[3] = from_f<T>(f1.y * sc);
+            o[2 * e] = reinterpret_cast<const uint32_t*>(&v)[0], o[2 * e + 1] = reinterpret_cast<const uint32_t*>(&v)[1];
+          }
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + t * cols + c), "r"(o[0]), "r"(o[1]), "r"(o[2]),
+                       "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7])
+                       : "memory");
+          continue;
+        }
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         Pack<T, 8> o;
@@ -510,11 +577,14 @@ int launch_norm(const NormArgs& a0, cudaStream_t st) {
   return check_launch("rms_norm_kernel");
 }
 
-// Two blocks a multiprocessor, fewer where a block would have less than four turns (each costs a partial row).
-int bwd_blocks(int64_t T, int rpc) {
+// As many blocks as a multiprocessor holds at 80 registers a thread (16384 x 4096 bf16, stages x blocks of 256 threads:
+// 3 x 2 124 us, 2 x 2 113, 2 x 3 103), fewer where a block would have less than four turns (each costs a partial row).
+constexpr int kBwdBlocks = 3;
+int bwd_blocks(int64_t T, int rpc, int threads) {
   const int64_t turns = ceil_div64(T, rpc), sms = multiprocessors();
+  const int per_sm = 256 * kBwdBlocks / threads < 1 ? 1 : (threads < 256 ? kBwdBlocks : 256 * kBwdBlocks / threads);
   int64_t blocks = turns / 4 < sms ? (turns < sms ? turns : sms) : turns / 4;
-  if (blocks > 2 * sms) blocks = 2 * sms;
+  if (blocks > per_sm * sms) blocks = per_sm * sms;
   return static_cast<int>(blocks);
 }
 
@@ -551,12 +621,12 @@ int bwd_for(NormBwdArgs a, void* dw, int dw_dtype, float* scratch, cudaStream_t 
                    (a.lddh * sizeof(T)) % 16 == 0 && (a.ldh * sizeof(T)) % 16 == 0;
   int e, per;
   row_shape(a.T, a.H, vec && a.T >= kManyRows ? 16 : 8, per, a.warps, a.rpc);
-  const int blocks = bwd_blocks(a.T, a.rpc);
+  const int blocks = bwd_blocks(a.T, a.rpc, a.rpc * a.warps * 32);
   if (vec) e = per == 8 ? launch_bwd<T, VE, 8 / VE>(a, blocks, st) : per == 16 ? launch_bwd<T, VE, 16 / VE>(a, blocks, st) : launch_bwd<T, VE, 32 / VE>(a, blocks, st);
   else e = per == 8 ? launch_bwd<T, 1, 8>(a, blocks, st) : per == 16 ? launch_bwd<T, 1, 16>(a, blocks, st) : launch_bwd<T, 1, 32>(a, blocks, st);
   if (e) return e;
   if (dw) {
-    norm_dw_kernel<<<ceil_div(a.H, 32), 256, 0, st>>>(scratch, blocks, a.H, dw, dw_dtype);
+    norm_dw_kernel<<<ceil_div(a.H, 32), 1024, 0, st>>>(scratch, blocks, a.H, dw, dw_dtype);
     return check_launch("norm_dw_kernel");
   }
   return 0;
@@ -627,7 +697,7 @@ extern "C" int omni_rms_norm(const void* x, int64_t ldx, const void* residual, i
 
 extern "C" size_t omni_rms_norm_bwd_scratch_bytes(int64_t rows, int hidden) {
   if (rows < 1 || hidden < 1 || hidden > kMaxHidden) return 0;
-  const int64_t most = 2 * static_cast<int64_t>(multiprocessors());
+  const int64_t most = kBwdBlocks * static_cast<int64_t>(multiprocessors());
   return sizeof(float) * static_cast<size_t>(rows < most ? rows : most) * hidden;
 }
 
@@ -642,7 +712,7 @@ extern "C" int omni_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, i
                omni_rms_norm_bwd_scratch_bytes(rows, hidden));
   NormBwdArgs a{};
   a.dy = dy, a.dh = dh, a.h = h, a.w = weight, a.lddy = lddy, a.lddh = dh ? lddh : 0, a.ldh = ldh, a.rstd = rstd;
-  a.w_f32 = w_dtype == OMNI_F32, a.T = rows, a.H = hidden, a.dx = dx, a.status = status;
+  a.w_f32 = w_dtype == OMNI_F32, a.T = rows, a.H = hidden, a.per_value = 1.f / hidden, a.dx = dx, a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* s = static_cast<float*>(scratch);
   if (dtype == OMNI_F32) return bwd_for<float>(a, dweight, w_dtype, s, st);
