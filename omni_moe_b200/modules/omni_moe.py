@@ -95,6 +95,7 @@ class OmniMoE(nn.Module):
 
         self._buffers_cache: dict = {}
         self._bn_cache = None
+        self._bn_pair = None
         self._checkpoint_bits = 16
         self.last_routing = None  # (scores, indices, weights) of the latest forward, for inspection
 
@@ -122,12 +123,25 @@ class OmniMoE(nn.Module):
         key = (bx.running_mean._version, bx.running_var._version, by.running_mean._version, by.running_var._version,
                bx.running_mean.data_ptr(), by.running_mean.data_ptr())
         if self._bn_cache is None or self._bn_cache[0] != key:
-            mean = torch.cat([bx.running_mean, by.running_mean]).float()
-            var = torch.cat([bx.running_var, by.running_var]).float()
-            eps = torch.cat([torch.full_like(bx.running_var, bx.eps, dtype=torch.float32),
-                             torch.full_like(by.running_var, by.eps, dtype=torch.float32)])
-            scale = torch.rsqrt(var + eps)
-            self._bn_cache = (key, scale.contiguous(), (-mean * scale).contiguous())
+            with torch.no_grad(), torch.inference_mode(False):  # ordinary tensors, whoever asks first
+                mean = torch.cat([bx.running_mean, by.running_mean]).float()
+                var = torch.cat([bx.running_var, by.running_var]).float()
+                eps = torch.cat([torch.full_like(bx.running_var, bx.eps, dtype=torch.float32),
+                                 torch.full_like(by.running_var, by.eps, dtype=torch.float32)])
+                scale = torch.rsqrt(var + eps)
+                shift = -mean * scale
+                if scale.is_cuda:
+                    if torch.cuda.is_current_stream_capturing():
+                        return scale, shift  # the graph's own memory, computed in every replay: not to be kept
+                    # once per change of the statistics: the pair keeps its address (graphs may hold it), no launch on any
+                    # stream still reads the old values, and every stream may read the new ones
+                    torch.cuda.synchronize(scale.device)
+                    pair = getattr(self, "_bn_pair", None)
+                    if pair is not None and pair[0].device == scale.device and pair[0].shape == scale.shape:
+                        scale, shift = pair[0].copy_(scale), pair[1].copy_(shift)
+                    torch.cuda.synchronize(scale.device)
+                    self._bn_pair = (scale, shift)
+                self._bn_cache = (key, scale, shift)
         return self._bn_cache[1], self._bn_cache[2]
 
     def sync_batch_statistics(self, group=None, enabled: bool = True) -> "OmniMoE":
@@ -378,7 +392,9 @@ class OmniMoE(nn.Module):
     def decode(self, hidden_states: torch.Tensor) -> torch.Tensor:
         """The eval-mode forward of at most 64 tokens ``[B, S, H]`` as one kernel (:func:`omni_decode_func`): the decode
         steps of a serving program.  The same definition as :meth:`forward`, another order of summation.  Allocates
-        only its output (and a per-stream workspace once), so it can be captured in a CUDA graph; inference only."""
+        only its output (and a per-stream workspace once), so it can be captured in a CUDA graph, best after one call
+        outside it (the BatchNorm fold of the running statistics is then not part of the graph, and replays see the
+        statistics of the module's latest call); inference only."""
         from ..ops.decode import omni_decode_func
         if self.training:
             raise RuntimeError("decode() uses the running statistics of the router's BatchNorm: call eval() first")

@@ -296,3 +296,61 @@ def test_ties_go_to_the_lower_index(t, n, k):
     assert clear.sum() >= t // 2
     off = (call(p).double() - terms.sum(1)).abs()
     assert (off <= bound)[clear].all()
+
+
+def layer():
+    from omni_moe_b200.modules.omni_moe import OmniMoE, OmniMoEConfig
+    torch.manual_seed(0)
+    m = OmniMoE(OmniMoEConfig(256, 512, "silu", 1024, 8)).bfloat16().cuda().eval()
+    return m, torch.randn(1, 5, 256, device="cuda").bfloat16()
+
+
+def move_statistics(m, to):
+    with torch.no_grad():
+        for bn in (m.router_norm_x, m.router_norm_y):
+            bn.running_mean.fill_(to)
+            bn.running_var.copy_(torch.linspace(0.5, 2.0, bn.running_var.numel()))
+
+
+def test_capture_before_the_first_call():
+    """The BatchNorm fold that a capture computes lives in the graph: calls outside must not read it."""
+    m, x = layer()
+    other, _ = layer()
+    want = other.decode(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(g):
+        out = m.decode(x)
+    assert torch.equal(m.decode(x), want)   # before any replay
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_statistics_that_change_between_replays():
+    m, x = layer()
+    m.decode(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(g):
+        out = m.decode(x)
+    for to in (0.25, -0.5):
+        move_statistics(m, to)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = m.decode(x)
+        again = m.decode(x)      # on another stream than the fold was computed on
+        junk = [torch.full((64,), float("nan"), device="cuda") for _ in range(64)]  # would land in memory given back
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, want) and torch.equal(out, want)
+        del junk
+
+
+def test_fold_made_in_inference_mode():
+    m, x = layer()
+    with torch.inference_mode():
+        m.decode(x)
+    move_statistics(m, 0.5)
+    fresh, _ = layer()
+    move_statistics(fresh, 0.5)
+    assert torch.equal(m.decode(x), fresh.decode(x))
