@@ -59,7 +59,15 @@ Tensor rows_of(const Tensor& t) {
   const bool whole = (m.size(1) == 1 || m.stride(1) == 1) && (m.size(0) <= 1 || m.stride(0) >= m.size(1));
   return whole ? m : m.contiguous();
 }
-Tensor as_bf16(const Tensor& t) { return t.to(at::kBFloat16).contiguous(); }
+// Contiguous bf16 on a 16-byte boundary, as the GEMMs' operands have to be.
+Tensor as_bf16(const Tensor& t) {
+  Tensor b = t.to(at::kBFloat16).contiguous();
+  return reinterpret_cast<uintptr_t>(b.data_ptr()) % 16 ? b.clone() : b;
+}
+// Backward passes here are not differentiable again: better an error than a second derivative of zero.
+void once(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative: run its backward without create_graph");
+}
 
 std::pair<Tensor, Tensor> empty_mx(int64_t rows, int64_t cols, const Tensor& like) {
   return {at::empty({rows, cols}, like.options().dtype(at::kFloat8_e4m3fn)),
@@ -151,6 +159,7 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("omni_rms_norm_func");
     const auto saved = ctx->get_saved_variables();
     const Tensor &h = saved[0], &weight = saved[1], &rstd = saved[2];
     // (the indices of needs_input_grad count the tensors that were given)
@@ -283,6 +292,7 @@ struct MlpCkptNode : torch::autograd::Function<MlpCkptNode> {
     return x.scalar_type() == at::kBFloat16 ? y : y.to(x.scalar_type());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("omni_mlp_ckpt_func");
     const auto s = ctx->get_saved_variables();
     OptTensor x;
     if (s.size() == 6) x = s[5];

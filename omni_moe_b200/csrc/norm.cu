@@ -491,7 +491,8 @@ template <typename T, int VE>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             int64_t rows, int cols, T* out) {
   const int scols = (cols + mx::kBlock - 1) / mx::kBlock;
-  const int c = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x) * VE;
+  // (64 bits: the last threads of a row of almost 2^31 values lie behind it)
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * VE;
   if (c >= cols) return;
 #pragma unroll 2
   for (int64_t t = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; t < rows; t += static_cast<int64_t>(gridDim.y) * blockDim.y) {
@@ -660,7 +661,7 @@ int dequantize_for(const uint8_t* codes, const uint8_t* scales, int64_t rows, in
   int bx = 32;
   while (bx < pieces && bx < 256) bx *= 2;
   const dim3 block(bx, 256 / bx);
-  const int64_t gx = ceil_div(pieces, bx), want = ceil_div64(rows, 2 * block.y);
+  const int64_t gx = ceil_div64(pieces, bx), want = ceil_div64(rows, 2 * block.y);
   OMNI_REQUIRE(gx < (int64_t(1) << 31), "too many columns");
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(want < 65535 ? want : 65535));
   if (vec) mx_dequantize_kernel<T, 16><<<grid, block, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));

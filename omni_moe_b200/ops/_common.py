@@ -12,6 +12,11 @@ def as_bf16(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t``, copied (differentiably) where its first value is not on a 16-byte boundary, which the GEMMs' operands need."""
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def pad_last(t: torch.Tensor, multiple: int = 8) -> torch.Tensor:
     """``t`` with its last dimension zero-padded up to a multiple (differentiable).  The kernels move
     rows in 16-byte pieces, i.e. want row lengths that are multiples of 8 bf16 elements; other lengths

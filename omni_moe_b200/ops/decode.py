@@ -5,10 +5,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._common import as_bf16, pad_both, pad_last
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+from ._common import aligned, as_bf16, pad_both, pad_last
 
 
 def omni_decode_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, down_weight: torch.Tensor,
@@ -46,5 +43,5 @@ def _prepared(tensors, k, bn_scale, bn_shift):
     h = x.size(1)
     # zero columns add nothing to a dot product and give output columns that are cut off again
     ready = (pad_last(x), pad_both(wg), pad_both(wu), pad_both(wd), pad_last(kx), pad_last(ky), pad_last(up), pad_last(down))
-    y = omni_decode_func(*(_aligned(v) for v in ready), k, bn_scale, bn_shift)
+    y = omni_decode_func(*(aligned(v) for v in ready), k, bn_scale, bn_shift)
     return (y if y.size(1) == h else y[:, :h].contiguous()).to(tensors[0].dtype)

@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._common import as_bf16, pad_both, pad_last
+from ._common import aligned, as_bf16, pad_both, pad_last
 from .mx import CODE_DTYPE, SCALE_DTYPE, mx_dequantize, mx_quantize, scale_columns
 
 
@@ -61,11 +61,12 @@ class MlpCkptCopiesFunction(torch.autograd.Function):
         return y.to(x.dtype)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         wg, wu, wd, codes, scales, xk, xs = ctx.saved_tensors
         need = ctx.needs_input_grad
         x = xk if ctx.keep_x else mx_dequantize(xk, xs)
-        grads = mlp_ckpt_backward(as_bf16(dy), x, codes, scales, wg, wu, wd, ctx.limit, need_x=need[0], need_gate_up=need[1] or need[2],
+        grads = mlp_ckpt_backward(aligned(as_bf16(dy)), x, codes, scales, wg, wu, wd, ctx.limit, need_x=need[0], need_gate_up=need[1] or need[2],
                                   need_down=need[3])
         return tuple(g.to(dt) if n and g is not None else None for g, dt, n in zip(grads, ctx.dtypes, need)) + (None,) * 4
 
@@ -117,7 +118,7 @@ def omni_mlp_ckpt_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: to
     if not (torch.is_grad_enabled() and (x.requires_grad or gate_weight.requires_grad or up_weight.requires_grad or down_weight.requires_grad)):
         from .mlp import mlp_forward
         x, gate_weight, up_weight, down_weight = (as_bf16(v) for v in tensors)
-        y = mlp_forward(pad_last(x), pad_both(gate_weight), pad_both(up_weight), pad_both(down_weight), limit=limit)
+        y = mlp_forward(*(aligned(v) for v in (pad_last(x), pad_both(gate_weight), pad_both(up_weight), pad_both(down_weight))), limit=limit)
         return (y[:, :h].contiguous() if padded else y).to(tensors[0].dtype)
     if padded:
         # zero columns: gate = up = 0 there, nothing is added and their gradients are cut off again; a block of 32 that is
@@ -125,6 +126,7 @@ def omni_mlp_ckpt_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: to
         if codes is not None:
             codes = pad_last(codes.view(torch.uint8)).view(CODE_DTYPE)
         x, gate_weight, up_weight, down_weight = pad_last(x), pad_both(gate_weight), pad_both(up_weight), pad_both(down_weight)
+    x, gate_weight, up_weight, down_weight = (aligned(v) for v in (x, gate_weight, up_weight, down_weight))
     from .autograd import _operands_in_place
     if _operands_in_place():
         y = _lib.binding().mlp_ckpt(x, gate_weight, up_weight, down_weight, float(limit or 0.0), codes, scales, bool(keep_x),

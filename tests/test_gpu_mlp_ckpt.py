@@ -255,3 +255,40 @@ def test_refusals():
             omni_mlp_ckpt_func(*args, **kw)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         omni_mlp_ckpt_func(x.cpu(), wg, wu, wd)
+
+
+@pytest.mark.parametrize("way", ["", "copies"])
+def test_operands_off_alignment(way, monkeypatch):
+    """Contiguous tensors that start between 16-byte boundaries, such as views into one flat buffer of parameters."""
+    from omni_moe_b200.ops import omni_mlp_ckpt_func
+    tensors, dy = make(40, 64, 96, 2)
+    leaves = [v.requires_grad_() for v in tensors]
+    if way:
+        monkeypatch.setenv("OMNI_MOE_B200_MLP_BWD", way)
+
+    def off(v):
+        return torch.cat((v.new_zeros(3), v.detach().flatten()))[3:].view(v.shape)
+
+    want = omni_mlp_ckpt_func(*leaves)
+    want_grads = torch.autograd.grad(want, leaves, dy)
+    moved = [off(v).requires_grad_() for v in leaves]
+    assert all(v.data_ptr() % 16 for v in moved)
+    got = omni_mlp_ckpt_func(*moved)
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        assert torch.equal(omni_mlp_ckpt_func(*moved), want)
+    for a, b in zip(torch.autograd.grad(got, moved, off(dy)), want_grads):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("way", ["", "copies"])
+def test_no_second_derivative(way, monkeypatch):
+    from omni_moe_b200.ops import omni_mlp_ckpt_func
+    tensors, _ = make(8, 64, 96, 2)
+    leaves = [v.requires_grad_() for v in tensors]
+    if way:
+        monkeypatch.setenv("OMNI_MOE_B200_MLP_BWD", way)
+    y = omni_mlp_ckpt_func(*leaves)
+    with pytest.raises(RuntimeError, match="no second derivative|once_differentiable"):
+        (dx,) = torch.autograd.grad(y.square().sum(), leaves[0], create_graph=True)
+        dx.sum().backward()

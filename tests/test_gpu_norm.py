@@ -344,3 +344,26 @@ def test_refusals():
         mx_dequantize(c, s[:, :1])
     with pytest.raises(ValueError, match="float8"):
         mx_dequantize(c.view(torch.uint8), s)
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 80, 2 ** 31 - 65])
+def test_mx_of_the_longest_rows(n):
+    """The last block of threads reaches past column 2^31."""
+    from omni_moe_b200.ops import mx_dequantize, mx_quantize
+    x = torch.zeros(1, n, device="cuda", dtype=torch.bfloat16)
+    x[0, -5000:] = rand((5000,), torch.bfloat16, 1)
+    codes, scales = mx_quantize(x)
+    out = mx_dequantize(codes, scales)
+    from_block = (n - 6000) // 32 * 32
+    ref, _ = mx_reference(x[:, from_block:])
+    assert torch.equal(out[:, from_block:].double(), ref)
+    assert not out[:, :from_block].view(torch.uint8)[:, ::1021].any()
+    assert out[0, :8].tolist() == [0.0] * 8
+
+
+def test_no_second_derivative():
+    from omni_moe_b200.ops import omni_rms_norm_func
+    x, w = rand((4, 64), torch.float32, 1).requires_grad_(), rand((64,), torch.float32, 2)
+    y = omni_rms_norm_func(x, w).y
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(y.square().sum(), x, create_graph=True)
