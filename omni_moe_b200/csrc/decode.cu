@@ -10,15 +10,16 @@
 //
 //   MLP      gate | up rows -> act  --[all act written]-->  down rows  -> + routed sum -> y
 //   experts  router rows -> logits  --[all logits written]-->  selection, k dots (a few blocks per token)
-//                                   --[all coefficients written]-->  this block's columns of every token's Down rows
+//                                   and those k Down rows, a block's share summed --[all partial sums written]-->
+//                                   added up for this block's columns
 //
 // The brackets are counters in global memory; every wait (on them and on barriers in shared memory) is bounded.  Two forms
 // of the products (the rule that picks one stands in omni_decode): "direct" streams the weights through registers into
 // mma.sync, "ring" by TMA through shared memory into tcgen05.mma.  The expert warps' code is the same in both.
 //
-// Measured (B200, CUDA graph; floor = bytes at 6547 GB/s): 1 token x 256 x 1024 13.8 us (latency: five dependent passes
-// through L2 and a cooperative launch), 1 x 1024 x 4096 17.3 us (floor 3.9), 8 x 4096 x 11008 56.6 us (42.6: 75 % of the
-// copy rate), 64 x 2048 x 8192 41.1 us (17.1), 24 x 4096 x 11008 with 64 of 2^20 experts 71.3 us (47.8).
+// Measured (B200, CUDA graph; floor = bytes at 6547 GB/s): 1 token x 256 x 1024 12.7 us (latency: five dependent passes
+// through L2 and a cooperative launch), 1 x 1024 x 4096 16.3 us (floor 3.9), 8 x 4096 x 11008 56.5 us (42.6: 75 % of the
+// copy rate), 64 x 2048 x 8192 40.4 us (17.1), 24 x 4096 x 11008 with 64 of 2^20 experts 69.6 us (47.8).
 // The layer's four-kernel forward takes as long for one token as for 256.
 //
 // act is rounded to bf16 (it is an operand of the down projection); everything else is summed in fp32 and y is rounded
@@ -41,7 +42,7 @@ constexpr int kSlots = 8;              // at most
 constexpr int kSlotBytes = 24 * 1024;  // at least
 constexpr int kSmemMost = 226 * 1024;  // dynamic shared memory of a block beside its static part
 // counters, one per 128-byte line
-enum { CNT_LOGITS = 0, CNT_ACT = 32, CNT_COEF = 64, CNT_EXIT = 96, CNT_GROUP = 128, kGroupStride = 8, kMaxGroups = 256,
+enum { CNT_LOGITS = 0, CNT_ACT = 32, CNT_ROUTED = 64, CNT_EXIT = 96, CNT_GROUP = 128, kGroupStride = 8, kMaxGroups = 256,
        CNT_WORDS = CNT_GROUP + kGroupStride * kMaxGroups };
 constexpr int kMaxSplit = 4;  // blocks of a group that cuts K
 
@@ -60,8 +61,7 @@ struct DecodeArgs {
   int m_r, m_gu, m_d;             // M of the tcgen05 tiles: 64 or 128
   int* counters;
   float* logits;   // [rsplit, T, 2n]: partial sums
-  float* coef;     // [T, k]
-  int* index;      // [T, k]
+  float* routed;   // [share, T, H]: partial routed sums
   __nv_bfloat16* act;  // [T, I]
   float* partial;  // [ksplit, T, H]
   __nv_bfloat16* y;
@@ -88,7 +88,7 @@ struct Share {
   int k0, k1;  // its K slices of the down projection
   int part;    // its place in the group
 };
-// Output columns go in groups of four: the Down rows are read in 8-byte pieces.
+// Output columns go in groups of four.
 __device__ __forceinline__ Share share_of(const DecodeArgs& a, int c, int G) {
   const auto cut = [](int64_t n, int i, int of) { return static_cast<int>(n * i / of); };
   Share s;
@@ -114,9 +114,9 @@ __device__ __forceinline__ Share share_of(const DecodeArgs& a, int c, int G) {
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// One thread, after a barrier of the threads whose writes it announces.
+// One thread, after a barrier of the threads whose writes it announces: the release covers them too (barriers are part of
+// the causality order).  A fence of its own in front of it would wait for the same writes twice.
 __device__ __forceinline__ void signal(int* counter) {
-  __threadfence();
   asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(counter) : "memory");
 }
 // Bounded: gives up after about two seconds, flags it, and lets the caller go on (its results are then invalid; every
@@ -692,8 +692,7 @@ __device__ __forceinline__ void select_by_block(const DecodeArgs& a, int t, Expe
 }
 
 // first_warp: the first of the kExpWarps warps that call this.  The code is kept small: it runs once a launch, and what
-// unrolling saves in latency it costs in instruction fetches (two rows of a dot product and three items of the last part
-// in flight instead of one: 12 us slower at 24 tokens x 4096).
+// unrolling saves in latency it costs in instruction fetches (two rows of a dot product in flight instead of one: slower).
 __device__ __forceinline__ void expert_path(const DecodeArgs& a, ExpertShared& sh, uint8_t* scratch, float* routed, const Share& b, int first_warp) {
   const int warp = (threadIdx.x >> 5) - first_warp, lane = lane_id();
   const int tid = threadIdx.x - 32 * first_warp;
@@ -708,7 +707,7 @@ __device__ __forceinline__ void expert_path(const DecodeArgs& a, ExpertShared& s
     for (int task = c; task < tasks; task += G) {
       const int t = task / a.share, part_id = task - t * a.share;
       select_by_block(a, t, sh, *reinterpret_cast<SelectScratch*>(scratch), tid);
-      // the Down rows of this block's ranks are asked into L2 now: every block will read a piece of them
+      // the Down rows of this block's ranks are asked into L2 now, for the sums after the dots
       {
         const int j = part_id + a.share * tid;
         if (j < k && sh.index[j] >= 0 && sh.index[j] < a.N) prefetch_l2(a.down + static_cast<int64_t>(sh.index[j]) * a.H, 2 * a.H);
@@ -743,72 +742,66 @@ __device__ __forceinline__ void expert_path(const DecodeArgs& a, ExpertShared& s
         dot = warp_sum(dot);
         if (lane == 0) {
           if (!ok) atomicOr(a.status, OMNI_ST_BAD_EXPERT_INDEX);
-          a.coef[static_cast<int64_t>(t) * k + j] = ok ? sh.weight[j] * silu(dot) : 0.f;
-          a.index[static_cast<int64_t>(t) * k + j] = ok ? e : 0;
+          sh.weight[j] = ok ? sh.weight[j] * silu(dot) : 0.f;
+          if (!ok) sh.index[j] = 0;
         }
       }
       bar_sync(2, kExpThreads);
-      if (tid == 0) signal(a.counters + CNT_COEF);
-    }
-  }
-  // this block's output columns of the routed sum of every token.  An item is (token, 4 columns); `lanes` lanes share
-  // one, each with up to eight of its ranks in flight.  The coefficients come through shared memory, as many tokens at a
-  // time as fit.
-  if (tid == 0) wait_for(a.counters + CNT_COEF, tasks, a.status);
-  bar_sync(2, kExpThreads);
-  const int quads = (b.r1 - b.r0) / 4;
-  if (quads == 0) return;
-  const int lanes = k <= 8 ? 1 : (k <= 16 ? 2 : (k <= 32 ? 4 : 8));
-  const int sub = tid & (lanes - 1), first = tid / lanes, step = kExpThreads / lanes;
-  const int batch = min(T, kScratchBytes / (8 * k));
-  float2* pair = reinterpret_cast<float2*>(scratch);  // (coefficient, expert as bits)
-  for (int t0 = 0; t0 < T; t0 += batch) {
-    const int tn = min(batch, T - t0);
-    for (int q = tid; q < tn * k; q += kExpThreads) {
-      const int64_t at = static_cast<int64_t>(t0) * k + q;
-      const int e = __ldcg(a.index + at);
-      const bool ok = e >= 0 && e < a.N;
-      pair[q] = make_float2(ok ? __ldcg(a.coef + at) : 0.f, __int_as_float(ok ? e : 0));
-    }
-    bar_sync(2, kExpThreads);
-    const int items = tn * quads;
+      // this share of the token's routed sum, 8 neighbouring columns a thread, 8 rows in flight.  (Whole rows in the block
+      // that has their coefficients: when every block read its own columns of the rows of all tokens, each row's page went
+      // through every multiprocessor: 17 us after the last coefficient at 24 tokens x 64 rows of 4096, so 4.)
+      const int mine = (k - part_id + a.share - 1) / a.share;
+      float* out = a.routed + (static_cast<int64_t>(part_id) * T + t) * a.H;
 #pragma unroll 1
-    for (int i0 = 0; i0 < items; i0 += step) {
-      const int item = i0 + first;
-      const bool live = item < items;
-      const int t = live ? item / quads : 0, col = (live ? item - t * quads : 0) * 4;
-      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+      for (int p = tid; p < H8; p += kExpThreads) {
+        float s[8] = {};
 #pragma unroll 1
-      for (int j0 = sub; j0 < k; j0 += 8 * lanes) {
-        float cf[8];
-        uint2 d[8];
+        for (int m = 0; m < mine; m += 8) {
+          uint4 d[8];
+          float cf[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int j = j0 + q * lanes;
-          const bool in = live && j < k;
-          const float2 pr = in ? pair[t * k + j] : make_float2(0.f, 0.f);
-          cf[q] = pr.x;
-          d[q] = in ? __ldg(reinterpret_cast<const uint2*>(a.down + static_cast<int64_t>(__float_as_int(pr.y)) * a.H + b.r0 + col)) : make_uint2(0, 0);
-        }
+          for (int q = 0; q < 8; ++q) {
+            const int j = part_id + a.share * (m + q);
+            const bool in = m + q < mine;
+            cf[q] = in ? sh.weight[j] : 0.f;
+            d[q] = in ? ldg128_stream(a.down + static_cast<int64_t>(sh.index[j]) * a.H + 8 * p) : make_uint4(0, 0, 0, 0);
+          }
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (live && j0 + q * lanes < k) {
-            const float2 lo = bf16x2_to_float2(d[q].x), hi = bf16x2_to_float2(d[q].y);
-            s0 = __fmaf_rn(cf[q], lo.x, s0), s1 = __fmaf_rn(cf[q], lo.y, s1), s2 = __fmaf_rn(cf[q], hi.x, s2), s3 = __fmaf_rn(cf[q], hi.y, s3);
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t dw[4] = {d[q].x, d[q].y, d[q].z, d[q].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = bf16x2_to_float2(dw[i]);
+              s[2 * i] = __fmaf_rn(cf[q], f.x, s[2 * i]), s[2 * i + 1] = __fmaf_rn(cf[q], f.y, s[2 * i + 1]);
+            }
           }
         }
+        __stcg(reinterpret_cast<float4*>(out + 8 * p), make_float4(s[0], s[1], s[2], s[3]));
+        __stcg(reinterpret_cast<float4*>(out + 8 * p) + 1, make_float4(s[4], s[5], s[6], s[7]));
       }
-#pragma unroll 1
-      for (int o = lanes / 2; o > 0; o >>= 1) {
-        s0 += __shfl_xor_sync(FULL_MASK, s0, o), s1 += __shfl_xor_sync(FULL_MASK, s1, o);
-        s2 += __shfl_xor_sync(FULL_MASK, s2, o), s3 += __shfl_xor_sync(FULL_MASK, s3, o);
-      }
-      if (live && sub == 0) {
-        float* o = routed + (t0 + t) * a.max_cols + col;
-        o[0] = s0, o[1] = s1, o[2] = s2, o[3] = s3;
-      }
+      bar_sync(2, kExpThreads);
+      if (tid == 0) signal(a.counters + CNT_ROUTED);
     }
-    bar_sync(2, kExpThreads);
+  }
+  // this block's output columns of every token, the shares added in order
+  if (tid == 0) wait_for(a.counters + CNT_ROUTED, tasks, a.status);
+  bar_sync(2, kExpThreads);
+  const int cols = b.r1 - b.r0;
+  const int64_t plane = static_cast<int64_t>(T) * a.H;
+#pragma unroll 1
+  for (int e = tid; e < T * cols; e += kExpThreads) {
+    const int t = e / cols, col = e - t * cols;
+    const float* p = a.routed + static_cast<int64_t>(t) * a.H + b.r0 + col;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int q0 = 0; q0 < a.share; q0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = q0 + q < a.share ? __ldcg(p + (q0 + q) * plane) : 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) sum += v[q];
+    }
+    routed[t * a.max_cols + col] = sum;
   }
 }
 
@@ -818,7 +811,7 @@ __device__ __forceinline__ void leave(const DecodeArgs& a) {
   if (threadIdx.x != 0) return;
   __threadfence();
   if (atomicAdd(a.counters + CNT_EXIT, 1) == static_cast<int>(gridDim.x) - 1) {
-    a.counters[CNT_LOGITS] = 0, a.counters[CNT_ACT] = 0, a.counters[CNT_COEF] = 0, a.counters[CNT_EXIT] = 0;
+    a.counters[CNT_LOGITS] = 0, a.counters[CNT_ACT] = 0, a.counters[CNT_ROUTED] = 0, a.counters[CNT_EXIT] = 0;
     if (a.ksplit > 1)
       for (int i = 0; i < a.groups; ++i) a.counters[CNT_GROUP + kGroupStride * i] = 0;
     __threadfence();
@@ -1205,6 +1198,11 @@ int launch_ring(DecodeArgs a, int sms, cudaStream_t st) {
   return launch_cooperative(decode_ring_kernel<N>, sms, kDecThreads, smem, st, tx, tkx, tky, tg, tu, td, ta, a);
 }
 
+// Blocks that work on one token's rows: as many as give each of a block's warps a row.
+int share_of_token(int num_tokens, int k) {
+  const int blocks = 148 / num_tokens, most = ceil_div(k, kExpWarps);
+  return blocks < 1 ? 1 : (blocks < most ? blocks : most);
+}
 int64_t round16(int64_t v) { return (v + 15) & ~int64_t(15); }
 bool is_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -1218,8 +1216,8 @@ extern "C" int omni_decode_max_tokens(void) { return kDecMaxTokens; }
 extern "C" size_t omni_decode_workspace_bytes(int num_tokens, int hidden, int intermediate, int sqrt_n, int k) {
   if (num_tokens < 1 || num_tokens > kDecMaxTokens || hidden < 8 || intermediate < 8 || sqrt_n < 1 || k < 1) return 0;
   const int64_t T = num_tokens;
-  return static_cast<size_t>(CNT_WORDS * 4 + round16(kMaxSplit * T * 2 * sqrt_n * 4) + 2 * round16(T * k * 4) + round16(T * intermediate * 2) +
-                             kMaxSplit * T * hidden * 4);
+  return static_cast<size_t>(CNT_WORDS * 4 + round16(kMaxSplit * T * 2 * sqrt_n * 4) + share_of_token(num_tokens, k) * T * hidden * 4 +
+                             round16(T * intermediate * 2) + kMaxSplit * T * hidden * 4);
 }
 
 extern "C" int omni_decode(const void* x, const void* gate_w, const void* up_w, const void* down_w, const void* router_x,
@@ -1252,27 +1250,23 @@ extern "C" int omni_decode(const void* x, const void* gate_w, const void* up_w, 
   a.T = num_tokens, a.H = hidden, a.I = intermediate, a.n = sqrt_n, a.k = k, a.kk = sqrt_n < k ? sqrt_n : k;
   a.cells = region_cells(a.kk, k);
   a.N = num_experts;
-  // blocks per token for the dot products: as many as give each of a block's warps a row
-  a.share = sms / num_tokens;
-  if (a.share > ceil_div(k, kExpWarps)) a.share = ceil_div(k, kExpWarps);
-  if (a.share < 1) a.share = 1;
+  a.share = share_of_token(num_tokens, k);
   uint8_t* w = static_cast<uint8_t*>(workspace);
   const int64_t T = num_tokens;
   a.counters = reinterpret_cast<int*>(w), w += CNT_WORDS * 4;
   a.logits = reinterpret_cast<float*>(w), w += round16(kMaxSplit * T * 2 * sqrt_n * 4);
-  a.coef = reinterpret_cast<float*>(w), w += round16(T * k * 4);
-  a.index = reinterpret_cast<int*>(w), w += round16(T * k * 4);
+  a.routed = reinterpret_cast<float*>(w), w += a.share * T * hidden * 4;
   a.act = reinterpret_cast<__nv_bfloat16*>(w), w += round16(T * intermediate * 2);
   a.partial = reinterpret_cast<float*>(w);
   a.y = static_cast<__nv_bfloat16*>(y), a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // The form.  Up to 8 tokens the direct one is the faster at every size (hidden x intermediate, direct / ring in us:
-  // 256 x 1024 13.8 / 19.1, 1024 x 4096 17.6 / 21.3, 4096 x 11008 56.7 / 65.8).  From 9 to 16 it has half the weights in
-  // flight and loses once a block has much to stream (1024 x 4096 19.5 / 22.4, 2048 x 5632 31.7 / 32.2, 2048 x 8192
-  // 42.1 / 40.0, 4096 x 11008 73.0 / 67.1); beyond, its token operand no longer fits the registers.
+  // 256 x 1024 13.8 / 17.5, 1024 x 4096 17.3 / 20.3, 2048 x 8192 31.8 / 33.1, 4096 x 11008 56.5 / 61.6).  From 9 to 16 it
+  // has half the weights in flight and loses once a block has much to stream (1024 x 4096, 0.17 MB a block, 18.7 / 20.6;
+  // 2048 x 5632, 0.48 MB, 31.4 / 28.0; 4096 x 11008 73.0 / 62.9); beyond, its token operand no longer fits the registers.
   const int64_t bytes = 2 * (3 * static_cast<int64_t>(intermediate) + 2 * sqrt_n) * hidden;
   if (num_tokens <= 8) return launch_direct<1>(a, sms, st);
-  if (num_tokens <= 16 && bytes <= sms * (int64_t(1) << 19)) return launch_direct<2>(a, sms, st);
+  if (num_tokens <= 16 && bytes <= sms * (int64_t(1) << 18)) return launch_direct<2>(a, sms, st);
   if (num_tokens <= 16) return launch_ring<16>(a, sms, st);
   if (num_tokens <= 32) return launch_ring<32>(a, sms, st);
   return launch_ring<64>(a, sms, st);

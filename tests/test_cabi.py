@@ -110,8 +110,8 @@ def test_decode_rejections(lib):
     assert call(t=0)[0] == 0  # nothing to do
     assert lib.omni_decode_max_tokens() == 64
     assert lib.omni_decode_workspace_bytes(65, 64, 64, 8, 4) == 0
-    # counters, partial logits, coefficients and indices, activation, partial sums of the down projection
-    assert lib.omni_decode_workspace_bytes(3, 24, 40, 5, 7) == 8704 + 4 * 3 * 10 * 4 + 2 * 96 + 240 + 4 * 3 * 24 * 4
+    # counters, partial logits, partial routed sums (one block a token here), activation, partial sums of the down projection
+    assert lib.omni_decode_workspace_bytes(3, 24, 40, 5, 7) == 8704 + 4 * 3 * 10 * 4 + 3 * 24 * 4 + 240 + 4 * 3 * 24 * 4
 
 
 def test_norm_and_mx_rejections(lib):
