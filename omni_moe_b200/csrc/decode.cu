@@ -474,8 +474,9 @@ __device__ __forceinline__ int rank_of(const uint32_t* all, int n, uint32_t mine
   return r;
 }
 
-// Cells (i+1)(j+1) <= k of the kk x kk grid in rank space, row by row (see router_select.cuh).
-__device__ __forceinline__ void fill_cells(ExpertShared& sh, int kk, int k, int tid) {
+// Cells (i+1)(j+1) <= k of the kk x kk grid in rank space, row by row (see router_select.cuh).  Returns the number of cells
+// in row tid (kk where there is no such row).
+__device__ __forceinline__ int fill_cells(ExpertShared& sh, int kk, int k, int tid) {
   const int lane = tid & 31;
   const int mine = tid < kk ? min(kk, k / (tid + 1)) : 0;  // kk <= 128: the first four warps
   int sum = mine;
@@ -492,6 +493,7 @@ __device__ __forceinline__ void fill_cells(ExpertShared& sh, int kk, int k, int 
 #pragma unroll 1
     for (int j = 0; j < mine; ++j) sh.cell[at + j] = static_cast<uint16_t>(tid | (j << 8));
   }
+  return tid < kk ? mine : kk;
 }
 
 // The same result from all kk x kk cells, by one warp: round after round the best entry that comes after the previous
@@ -533,7 +535,8 @@ __device__ __noinline__ void select_exactly(int n, int k, int kk, ExpertShared& 
 // its own, which has no dependency chain.  With more than 128 entries an axis is thinned first: the kk-th largest of the
 // 128 threads' maxima is a lower bound of the kk-th largest entry, and few more entries reach it.  Leaves the selection
 // in sh.index / sh.weight, ending with a barrier.
-__device__ __forceinline__ void select_by_block(const DecodeArgs& a, int t, ExpertShared& sh, SelectScratch& w, int tid) {
+// j0: column of the first cell outside the pruned region in row tid, kk or more where there is none.
+__device__ __forceinline__ void select_by_block(const DecodeArgs& a, int t, ExpertShared& sh, SelectScratch& w, int tid, int j0) {
   const int axis = tid >> 7, i = tid & 127, lane = tid & 31, quad = (tid >> 5) & 3;
   const int n = a.n, k = a.k, kk = a.kk;
   const int64_t plane = static_cast<int64_t>(a.T) * (2 * n);
@@ -677,18 +680,13 @@ __device__ __forceinline__ void select_by_block(const DecodeArgs& a, int t, Expe
     }
     bar_sync(2, kExpThreads);
     const bool missing = (i < kk && sh.idx[axis][i] < 0) || (tid < k && sh.index[tid] < 0);
+    // a cell outside the pruned region that ties with the last score
+    const bool odd = j0 < kk && float_to_key(__fadd_rn(sh.val[0][tid], sh.val[1][j0])) >= sh.last;
+    if (!bar_any(2, kExpThreads, missing || odd)) return;
     if (!bar_any(2, kExpThreads, missing)) break;
   }
-  // a cell outside the pruned region that ties with the last score (or keys that are no numbers)
-  bool odd = (i < kk && sh.idx[axis][i] < 0) || (tid < k && sh.index[tid] < 0);
-  if (tid < kk) {
-    const int j0 = min(kk, k / (tid + 1));
-    odd |= j0 < kk && float_to_key(__fadd_rn(sh.val[0][tid], sh.val[1][j0])) >= sh.last;
-  }
-  if (bar_any(2, kExpThreads, odd)) {
-    if (tid < 32) select_exactly(n, k, kk, sh, w);
-    bar_sync(2, kExpThreads);
-  }
+  if (tid < 32) select_exactly(n, k, kk, sh, w);
+  bar_sync(2, kExpThreads);
 }
 
 // first_warp: the first of the kExpWarps warps that call this.  The code is kept small: it runs once a launch, and what
@@ -701,12 +699,12 @@ __device__ __forceinline__ void expert_path(const DecodeArgs& a, ExpertShared& s
   // selection and dot products: `share` blocks per token, each selects (the same routing) and takes every share-th rank
   const int tasks = T * a.share;
   if (c < tasks) {
-    fill_cells(sh, a.kk, k, tid);
+    const int j0 = fill_cells(sh, a.kk, k, tid);
     if (tid == 0) wait_for(a.counters + CNT_LOGITS, G, a.status);
     bar_sync(2, kExpThreads);
     for (int task = c; task < tasks; task += G) {
       const int t = task / a.share, part_id = task - t * a.share;
-      select_by_block(a, t, sh, *reinterpret_cast<SelectScratch*>(scratch), tid);
+      select_by_block(a, t, sh, *reinterpret_cast<SelectScratch*>(scratch), tid, j0);
       // the Down rows of this block's ranks are asked into L2 now, for the sums after the dots
       {
         const int j = part_id + a.share * tid;
