@@ -17,9 +17,9 @@
 // of the products (the rule that picks one stands in omni_decode): "direct" streams the weights through registers into
 // mma.sync, "ring" by TMA through shared memory into tcgen05.mma.  The expert warps' code is the same in both.
 //
-// Measured (B200, CUDA graph; floor = bytes at 6547 GB/s): 1 token x 256 x 1024 12.7 us (latency: five dependent passes
-// through L2 and a cooperative launch), 1 x 1024 x 4096 16.3 us (floor 3.9), 8 x 4096 x 11008 56.5 us (42.6: 75 % of the
-// copy rate), 64 x 2048 x 8192 40.4 us (17.1), 24 x 4096 x 11008 with 64 of 2^20 experts 69.6 us (47.8).
+// Measured (B200, CUDA graph; floor = bytes at 6547 GB/s): 1 token x 256 x 1024 12.2 us (latency: five dependent passes
+// through L2 and a cooperative launch), 1 x 1024 x 4096 15.8 us (floor 3.9), 8 x 4096 x 11008 56.5 us (42.6: 75 % of the
+// copy rate), 64 x 2048 x 8192 40.4 us (17.1), 24 x 4096 x 11008 with 64 of 2^20 experts 69.5 us (47.8).
 // The layer's four-kernel forward takes as long for one token as for 256.
 //
 // act is rounded to bf16 (it is an operand of the down projection); everything else is summed in fp32 and y is rounded
