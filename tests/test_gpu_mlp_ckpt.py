@@ -292,3 +292,20 @@ def test_no_second_derivative(way, monkeypatch):
     with pytest.raises(RuntimeError, match="no second derivative|once_differentiable"):
         (dx,) = torch.autograd.grad(y.square().sum(), leaves[0], create_graph=True)
         dx.sum().backward()
+
+
+def test_more_values_than_32_bits_count():
+    """The last rows of 2^32 codes and more: the same bits as on their own (no sum runs over rows in what is compared)."""
+    from omni_moe_b200.ops import omni_mlp_ckpt_func
+    t, h, i, tail = 2 ** 17 + 5, 64, 2 ** 14 + 8, 5
+    tensors, _ = make(tail, h, i, 4)
+    last = tensors[0].clone().requires_grad_()
+    x = torch.zeros(t, h, device="cuda", dtype=torch.bfloat16)
+    x[-tail:] = tensors[0]
+    x.requires_grad_()
+    dy = torch.zeros_like(x)
+    dy[-tail:] = 1
+    big, small = omni_mlp_ckpt_func(x, *tensors[1:]), omni_mlp_ckpt_func(last, *tensors[1:])
+    assert torch.equal(big[-tail:], small) and not big[:-tail].any()
+    (dx,), (want,) = torch.autograd.grad(big, x, dy), torch.autograd.grad(small, last, dy[-tail:])
+    assert torch.equal(dx[-tail:], want) and not dx[:-tail].any()

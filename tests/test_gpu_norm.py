@@ -367,3 +367,24 @@ def test_no_second_derivative():
     y = omni_rms_norm_func(x, w).y
     with pytest.raises(RuntimeError, match="no second derivative"):
         torch.autograd.grad(y.square().sum(), x, create_graph=True)
+
+
+def test_more_values_than_32_bits_count():
+    """The last rows of 2^31 values and more: the same bits as on their own."""
+    from omni_moe_b200.ops import mx_dequantize, omni_rms_norm_func
+    t, n, tail = 2 ** 17 + 9, 16384, 9
+    x = torch.zeros(t, n, device="cuda", dtype=torch.bfloat16)
+    x[-tail:] = rand((tail, n), torch.bfloat16, 1)
+    w = rand((n,), torch.bfloat16, 2).requires_grad_()
+    last = x[-tail:].clone().requires_grad_()
+    x.requires_grad_()
+    dy = torch.zeros_like(x)
+    dy[-tail:] = rand((tail, n), torch.bfloat16, 3)
+    big, small = omni_rms_norm_func(x, w, quantize=True), omni_rms_norm_func(last, w, quantize=True)
+    assert torch.equal(big.y[-tail:], small.y) and not big.y[-tail - 1].any()
+    assert torch.equal(mx_dequantize(big.codes, big.scales)[-tail:], mx_dequantize(small.codes, small.scales))
+    dx, dw = torch.autograd.grad(big.y, (x, w), dy)
+    want, dw_want = torch.autograd.grad(small.y, (last, w), dy[-tail:])
+    # (rows of another number go to other threads: the sums of a row are ordered differently)
+    assert ((dx[-tail:].double() - want.double()).abs() <= 2 * half_step(torch.bfloat16) * want.double().abs() + 1e-5 * want.double().abs().max()).all()
+    assert ((dw.double() - dw_want.double()).abs() <= 2 * half_step(torch.bfloat16) * dw_want.double().abs() + 1e-5 * dw_want.double().abs().max()).all()
