@@ -117,32 +117,47 @@ class OmniMoE(nn.Module):
             w = w.to(torch.bfloat16)  # fp32 / fp16 modules: operands are rounded to bf16 per call
         return w.contiguous()
 
+    def _bn_fold_values(self):
+        bx, by = self.router_norm_x, self.router_norm_y
+        mean = torch.cat([bx.running_mean, by.running_mean]).float()
+        var = torch.cat([bx.running_var, by.running_var]).float()
+        eps = torch.cat([torch.full_like(bx.running_var, bx.eps, dtype=torch.float32),
+                         torch.full_like(by.running_var, by.eps, dtype=torch.float32)])
+        scale = torch.rsqrt(var + eps)
+        return scale.contiguous(), (-mean * scale).contiguous()
+
     def _bn_fold_eval(self):
         """Eval-mode BatchNorm of both axes as one scale / shift pair per logit column."""
         bx, by = self.router_norm_x, self.router_norm_y
         key = (bx.running_mean._version, bx.running_var._version, by.running_mean._version, by.running_var._version,
                bx.running_mean.data_ptr(), by.running_mean.data_ptr())
         if self._bn_cache is None or self._bn_cache[0] != key:
-            with torch.no_grad(), torch.inference_mode(False):  # ordinary tensors, whoever asks first
-                mean = torch.cat([bx.running_mean, by.running_mean]).float()
-                var = torch.cat([bx.running_var, by.running_var]).float()
-                eps = torch.cat([torch.full_like(bx.running_var, bx.eps, dtype=torch.float32),
-                                 torch.full_like(by.running_var, by.eps, dtype=torch.float32)])
-                scale = torch.rsqrt(var + eps)
-                shift = -mean * scale
-                if scale.is_cuda:
-                    if torch.cuda.is_current_stream_capturing():
-                        return scale, shift  # the graph's own memory, computed in every replay: not to be kept
-                    # once per change of the statistics: the pair keeps its address (graphs may hold it), no launch on any
-                    # stream still reads the old values, and every stream may read the new ones
-                    torch.cuda.synchronize(scale.device)
-                    pair = getattr(self, "_bn_pair", None)
-                    if pair is not None and pair[0].device == scale.device and pair[0].shape == scale.shape:
-                        scale, shift = pair[0].copy_(scale), pair[1].copy_(shift)
-                    torch.cuda.synchronize(scale.device)
-                    self._bn_pair = (scale, shift)
-                self._bn_cache = (key, scale, shift)
+            fold = self._bn_fold_values()
+            if fold[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                return fold  # the graph's own memory, computed in every replay: not to be kept
+            self._bn_cache = (key, *fold)
         return self._bn_cache[1], self._bn_cache[2]
+
+    def _bn_fold_decode(self):
+        """The same pair for :meth:`decode`, at an address that stays (graphs may hold it) and ready for calls on any stream."""
+        scale, shift = self._bn_fold_eval()
+        pair = getattr(self, "_bn_pair", None)  # (the tensor it was copied from, scale, shift)
+        if pair is not None and pair[0] is scale:
+            return pair[1], pair[2]
+        if torch.cuda.is_current_stream_capturing():
+            kept = self._bn_cache is not None and self._bn_cache[1] is scale
+            return self._bn_fold_values() if kept else (scale, shift)  # part of the graph
+        with torch.no_grad(), torch.inference_mode(False):  # ordinary tensors, whoever asks first
+            # once per change of the statistics: no launch on any stream still reads the old values afterwards, and every
+            # stream may read the new ones
+            torch.cuda.synchronize(scale.device)
+            if pair is not None and pair[1].device == scale.device and pair[1].shape == scale.shape:
+                pair[1].copy_(scale), pair[2].copy_(shift)
+                self._bn_pair = (scale, pair[1], pair[2])
+            else:
+                self._bn_pair = (scale, scale.clone(), shift.clone())
+            torch.cuda.synchronize(scale.device)
+        return self._bn_pair[1], self._bn_pair[2]
 
     def sync_batch_statistics(self, group=None, enabled: bool = True) -> "OmniMoE":
         """Training-mode BatchNorm over the tokens of every rank of ``group`` (default: all ranks), for
@@ -402,7 +417,7 @@ class OmniMoE(nn.Module):
         operands = self._operands()
         if hidden_states.dim() != 3 or hidden_states.size(2) != self.hidden_size:
             raise ValueError(f"hidden_states must be (batch, sequence, {self.hidden_size}), got {tuple(hidden_states.shape)}")
-        y = omni_decode_func(hidden_states.reshape(-1, self.hidden_size), *operands, self.top_k, *self._bn_fold_eval())
+        y = omni_decode_func(hidden_states.reshape(-1, self.hidden_size), *operands, self.top_k, *self._bn_fold_decode())
         self.last_status = _lib.device_status(hidden_states.device)
         return y.view(hidden_states.shape)
 

@@ -354,3 +354,37 @@ def test_fold_made_in_inference_mode():
     fresh, _ = layer()
     move_statistics(fresh, 0.5)
     assert torch.equal(m.decode(x), fresh.decode(x))
+
+
+def test_statistics_that_change_before_a_backward():
+    """What an eval-mode graph has kept of the statistics stays as it was when decode() follows new ones."""
+    m, x = layer()
+    grads = []
+    for decode in (False, True):
+        move_statistics(m, 0.25)
+        leaf = x.clone().requires_grad_()
+        y = m(leaf)
+        if decode:
+            m.decode(x)
+            move_statistics(m, -0.5)
+            m.decode(x), m(x)
+        grads.append(torch.autograd.grad(y.float().square().sum(), leaf)[0])
+    assert torch.equal(*grads)
+
+
+def test_capture_after_the_forward_alone():
+    m, x = layer()
+    with torch.no_grad():
+        m(x)
+        want = layer()[0].decode(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = m.decode(x)
+    move_statistics(m, 0.25)   # the fold that the forward made goes
+    m(x)
+    changed = m.decode(x)
+    junk = [torch.full((64,), float("nan"), device="cuda") for _ in range(64)]
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, changed) and not torch.equal(want, changed)
+    del junk
