@@ -573,7 +573,8 @@ OMNI_API int omni_rms_norm_bwd(const void *dy, int64_t lddy, const void *dh, int
  *   codes [rows, cols] e4m3 bytes;  scales [rows, ceil(cols / 32)] e8m0 bytes: byte b stands for 2^(b - 127), the
  *   smallest (b >= 0) for which the block's largest finite magnitude is <= 448 * 2^(b - 127)
  *   code = v / scale to nearest, ties to even; a value that is not finite becomes NaN and does not count for the scale
- * omni_mx_dequantize writes the values the codes stand for (exact where the type's range holds them).  Outputs are contiguous.
+ * omni_mx_dequantize writes the values the codes stand for (exact where the type's range holds them; NaN where the byte
+ * is 255, which omni_mx_quantize never writes).  Outputs are contiguous.
  */
 OMNI_API int omni_mx_quantize(const void *x, int64_t ldx, int dtype, int64_t rows, int64_t cols, void *codes, void *scales,
                               void *stream);

@@ -283,7 +283,7 @@ __device__ __forceinline__ void store_tile_dswiglu(uint32_t taddr, int row, int 
     for (int i = 0; i < 32; ++i) d[i] = __uint_as_float(ra[i]);
     if (ch + 1 < NCH) tmem_ld32_async(taddr + c + 32, ra);
     if (row < g.M && col0 < g.N) {
-      const float fg = mx::pow2(static_cast<int>((scales.g >> (8 * ch)) & 0xff) - 127), fu = mx::pow2(static_cast<int>((scales.u >> (8 * ch)) & 0xff) - 127);
+      const float fg = mx::scale_of((scales.g >> (8 * ch)) & 0xff), fu = mx::scale_of((scales.u >> (8 * ch)) & 0xff);
       __nv_bfloat16* og = reinterpret_cast<__nv_bfloat16*>(g.gu_out) + static_cast<int64_t>(row) * (2 * g.N) + col0;
       __nv_bfloat16* oa = reinterpret_cast<__nv_bfloat16*>(g.act_out) + static_cast<int64_t>(row) * g.N + col0;
 #pragma unroll

@@ -28,6 +28,8 @@ __device__ __forceinline__ int exponent_of(float top) {
 __device__ __forceinline__ float pow2(int s) {  // 2^s, -127 <= s <= 127
   return s == -127 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(s + 127) << 23);
 }
+// The scale that byte b stands for: 2^(b - 127), and NaN for 255, which no block of ours holds but others may.
+__device__ __forceinline__ float scale_of(uint32_t b) { return __uint_as_float(b == 0 ? 0x00400000u : b == 255 ? 0x7fffffffu : b << 23); }
 
 // Codes of two values (the first in the low byte); inv = 2^-s.  v - v is 0 for a finite v and NaN otherwise.
 __device__ __forceinline__ uint32_t encode2(float v0, float v1, float inv) {

@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
 #pragma unroll 2
   for (int64_t t = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; t < rows; t += static_cast<int64_t>(gridDim.y) * blockDim.y) {
     const uint8_t* p = codes + t * cols + c;
-    const float sc = mx::pow2(static_cast<int>(__ldg(scales + t * scols + c / mx::kBlock)) - 127);
+    const float sc = mx::scale_of(__ldg(scales + t * scols + c / mx::kBlock));
     if constexpr (VE == 16) {
       const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
       const uint32_t w[4] = {q.x, q.y, q.z, q.w};

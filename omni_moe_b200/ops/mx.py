@@ -25,5 +25,6 @@ def mx_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that the codes stand for: exact wherever the type's range holds them (a code may stand for up to 2^128:
-    infinite in bf16 and fp32; fp16 overflows and underflows earlier)."""
+    infinite in bf16 and fp32; fp16 overflows and underflows earlier).  Scale byte 255 stands for NaN,
+    as in ``torch.float8_e8m0fnu``; :func:`mx_quantize` never gives it."""
     return _lib.binding().mx_dequantize(codes, scales, dtype)

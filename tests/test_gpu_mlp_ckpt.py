@@ -309,3 +309,35 @@ def test_more_values_than_32_bits_count():
     assert torch.equal(big[-tail:], small) and not big[:-tail].any()
     (dx,), (want,) = torch.autograd.grad(big, x, dy), torch.autograd.grad(small, last, dy[-tail:])
     assert torch.equal(dx[-tail:], want) and not dx[:-tail].any()
+
+
+@pytest.mark.parametrize("limit", [0.0, 0.8])
+@pytest.mark.parametrize("i", [128, 96, 40])   # scales read as one word, byte by byte, and with a block that ends early
+def test_scale_that_is_no_number(i, limit):
+    """Scale byte 255 stands for NaN: the block's gradients and activation are NaN, all others stay."""
+    from omni_moe_b200 import _lib
+    (x, wg, wu, wd), dy = make(5, 64, i, 4)
+    _, codes, scales = forward(x, wg, wu, limit)
+    b = -(-i // 32)
+
+    def start(scales):
+        dgu, act = (torch.empty(5, c, device="cuda", dtype=torch.bfloat16) for c in (2 * i, i))
+        _lib.check(_lib.load().omni_mlp_dact_swiglu_mx(dy.data_ptr(), wd.data_ptr(), 5, 64, i, codes.data_ptr(), scales.data_ptr(), limit,
+                                                       dgu.data_ptr(), act.data_ptr(), _lib.device_status("cuda").data_ptr(), _lib.stream_ptr()))
+        _lib.check_device_status()
+        return dgu[:, :i], dgu[:, i:], act
+
+    clean = start(scales)
+    bad = scales.view(torch.uint8).clone()
+    bad[1, b - 1] = 255       # the last block of the gate's row 1
+    bad[3, b] = 255           # the first block of the up's row 3
+    gate, up = (torch.zeros(5, i, device="cuda", dtype=torch.bool) for _ in range(2))
+    gate[1, 32 * (b - 1):] = True
+    up[3, :32] = True
+    # a gate beyond the clamp passes no gradient, whatever up is, and the other way round; dup does not depend on up's value,
+    # but whether it is cut off does (for NaN it is not)
+    within = [v.abs() <= limit if limit else torch.ones_like(up) for v in decoded(codes, scales)]
+    cut = up & ~within[1]
+    for got, was, nan, same in zip(start(bad), clean, (gate | (up & within[0]), gate & within[1], gate | up), (torch.ones_like(cut), ~cut, torch.ones_like(cut))):
+        assert torch.isfinite(was).all()
+        assert got[nan].isnan().all() and torch.isfinite(got[~nan]).all() and torch.equal(got[~nan & same], was[~nan & same])

@@ -388,3 +388,20 @@ def test_more_values_than_32_bits_count():
     # (rows of another number go to other threads: the sums of a row are ordered differently)
     assert ((dx[-tail:].double() - want.double()).abs() <= 2 * half_step(torch.bfloat16) * want.double().abs() + 1e-5 * want.double().abs().max()).all()
     assert ((dw.double() - dw_want.double()).abs() <= 2 * half_step(torch.bfloat16) * dw_want.double().abs() + 1e-5 * dw_want.double().abs().max()).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [64, 48, 33])
+def test_every_scale_byte(cols, dtype):
+    """A scale byte b stands for 2^(b - 127), 255 for NaN: blocks may come from elsewhere than mx_quantize."""
+    from omni_moe_b200.ops import mx_dequantize
+    b = -(-cols // 32)
+    byte = torch.arange(256 * b, device="cuda").view(256, b) % 256
+    codes = (torch.arange(256 * cols, device="cuda").view(256, cols) * 37 % 127).to(torch.uint8)  # finite, both kinds of exponent
+    got = mx_dequantize(codes.view(torch.float8_e4m3fn), byte.to(torch.uint8).view(torch.float8_e8m0fnu), dtype)
+    c = codes.long()
+    value = torch.where(c < 8, c.double() / 8, (1 + (c % 8).double() / 8) * pow2((c // 8) - 1)) * 2.0 ** -6  # e4m3, from its definition
+    scale = pow2(byte - 127).masked_fill(byte == 255, float("nan")).repeat_interleave(32, 1)[:, :cols]
+    want = (value * scale).to(dtype)
+    assert torch.equal(got.isnan(), (byte == 255).repeat_interleave(32, 1)[:, :cols])
+    assert torch.equal(got.nan_to_num(nan=0.0, posinf=float("inf")), want.nan_to_num(nan=0.0, posinf=float("inf")))
