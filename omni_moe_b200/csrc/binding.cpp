@@ -364,8 +364,11 @@ OptTensor decode(const Tensor& x, const Tensor& gate, const Tensor& up, const Te
                         "bn_scale and bn_shift must be float32 vectors of 2 * sqrt_n values on the device of x");
     scale = bn_scale->contiguous(), shift = bn_shift->contiguous();
   }
-  TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()),
-              "omni_decode_func has no backward: call it under torch.no_grad(), or OmniMoE.forward to train");
+  if (at::GradMode::is_enabled()) {
+    bool leaf = (bn_scale && bn_scale->requires_grad()) || (bn_shift && bn_shift->requires_grad());
+    for (const Tensor* m : all) leaf = leaf || m->requires_grad();
+    TORCH_CHECK(!leaf, "omni_decode_func has no backward: call it under torch.no_grad(), or OmniMoE.forward to train");
+  }
   if (h % 8 || i % 8) return std::nullopt;
   for (const Tensor* m : all)
     if (m->scalar_type() != at::kBFloat16 || !m->is_contiguous() || reinterpret_cast<uintptr_t>(m->data_ptr()) % 16) return std::nullopt;

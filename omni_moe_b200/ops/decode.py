@@ -25,8 +25,8 @@ def omni_decode_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
     :param bn_scale, bn_shift: (2 * sqrt_n,) float32, x axis first; both or neither
     :return y: (num_tokens, hidden_size), dtype of ``x``
 
-    Operands are bf16 (others are rounded to it per call), sums fp32.  Inference only: a call whose ``x`` carries a
-    graph is refused.  Device-side faults are reported by ``check_device_status``.
+    Operands are bf16 (others are rounded to it per call), sums fp32.  Inference only: with gradients enabled, a call with a
+    tensor that requires them is refused.  Device-side faults are reported by ``check_device_status``.
     """
     k = int(num_experts_per_token)
     y = _lib.binding().decode(x, gate_weight, up_weight, down_weight, router_x, router_y, up_embed, down_embed, k, bn_scale, bn_shift,

@@ -388,3 +388,18 @@ def test_capture_after_the_forward_alone():
     torch.cuda.synchronize()
     assert torch.equal(out, changed) and not torch.equal(want, changed)
     del junk
+
+
+def test_weights_that_require_gradients_are_refused():
+    """With gradients enabled a result without a graph would train nothing, in silence."""
+    p = make(3, 64, 64, 8, 4, 1)
+    want = call(p)
+    for name in ("wg", "wu", "wd", "kx", "ky", "up", "down", "scale", "shift"):
+        leaf = p[name].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(p, **{name: leaf})
+        with torch.no_grad():
+            assert torch.equal(call(p, **{name: leaf}), want)
+    odd = make(3, 60, 64, 8, 4, 1)   # sizes that are padded first
+    with pytest.raises(RuntimeError, match="no backward"):
+        call(odd, wg=odd["wg"].clone().requires_grad_())
