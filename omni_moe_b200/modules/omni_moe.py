@@ -410,9 +410,12 @@ class OmniMoE(nn.Module):
         only its output (and a per-stream workspace once), so it can be captured in a CUDA graph, best after one call
         outside it (the BatchNorm fold of the running statistics is then not part of the graph, and replays see the
         statistics of the module's latest call); inference only."""
+        from ..ops._common import in_dual_level, refuse_tangents
         from ..ops.decode import omni_decode_func
         if self.training:
             raise RuntimeError("decode() uses the running statistics of the router's BatchNorm: call eval() first")
+        if in_dual_level():
+            refuse_tangents("OmniMoE.decode", hidden_states, *self.parameters(), *self.buffers())
         _lib.require_cuda(hidden_states)
         operands = self._operands()
         if hidden_states.dim() != 3 or hidden_states.size(2) != self.hidden_size:

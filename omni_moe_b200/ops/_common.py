@@ -2,6 +2,19 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
+
+
+def in_dual_level() -> bool:
+    """Whether tensors can have forward-mode derivatives at all."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def refuse_tangents(name: str, *tensors) -> None:
+    """Raises for tensors with a forward-mode derivative (``None`` entries are skipped): the kernels carry none, and an output
+    without one would pass for a derivative of zero."""
+    if in_dual_level() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def as_bf16(t: torch.Tensor) -> torch.Tensor:

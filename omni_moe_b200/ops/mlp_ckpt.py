@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._common import aligned, as_bf16, pad_both, pad_last
+from ._common import aligned, as_bf16, pad_both, pad_last, refuse_tangents
 from .mx import CODE_DTYPE, SCALE_DTYPE, mx_dequantize, mx_quantize, scale_columns
 
 
@@ -94,6 +94,7 @@ def omni_mlp_ckpt_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: to
     Operands other than bf16 are rounded to it; sums are fp32.
     """
     tensors = (x, gate_weight, up_weight, down_weight)
+    refuse_tangents("omni_mlp_ckpt_func", *tensors)
     _lib.require_cuda(*tensors)
     if x.dim() != 2 or gate_weight.dim() != 2:
         raise ValueError("omni_mlp_ckpt_func takes matrices")

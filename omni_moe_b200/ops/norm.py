@@ -7,6 +7,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
+from ._common import refuse_tangents
 
 
 class RmsNormOutput(NamedTuple):
@@ -33,4 +34,5 @@ def omni_rms_norm_func(x: torch.Tensor, weight: torch.Tensor, residual: Optional
 
     Sums are fp32.  Differentiable in ``x``, ``residual`` and ``weight``; the weight's gradient is summed in a fixed order.
     """
+    refuse_tangents("omni_rms_norm_func", x, weight, residual)
     return RmsNormOutput(*_lib.binding().rms_norm(x, weight, residual, float(eps), bool(quantize), _lib.status_ptr(x)))

@@ -66,3 +66,18 @@ def test_block_parameters():
     assert "norm.weight" in names and "layer.gate_proj.weight" in names and b.norm.weight.shape == (64,) and b.norm.eps == 1e-5
     with pytest.raises(ValueError, match="8 or 16"):
         OmniMoEBlock(OmniMoEConfig(64, 128, "silu", 256, 4), checkpoint_bits=32)
+
+
+def test_forward_mode_is_seen_before_anything_runs():
+    """Dual tensors and those of torch.func.jvp, which wraps them."""
+    import torch.autograd.forward_ad as fw
+    from omni_moe_b200 import ops
+    x, w = torch.ones(4, 64), torch.ones(64)
+    calls = (lambda v: ops.omni_rms_norm_func(v, w).y, lambda v: ops.omni_mlp_ckpt_func(v, v, v, v), lambda v: ops.omni_decode_func(*[v] * 8, 4))
+    for call in calls:
+        with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(fw.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
+        with fw.dual_level(), pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call(x)

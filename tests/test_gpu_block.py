@@ -125,3 +125,54 @@ def test_checkpoint_bits_are_checked():
     assert m.checkpoint_activations(8) is m
     with pytest.raises(ValueError, match="8 or 16"):
         m.checkpoint_activations(4)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """The kernels carry no tangents: an output without one would be a derivative of zero."""
+    from omni_moe_b200.modules import OmniMoE, OmniMoEBlock, OmniMoEConfig
+    from omni_moe_b200.ops import omni_decode_func, omni_mlp_ckpt_func, omni_rms_norm_func
+    import torch.autograd.forward_ad as fw
+    torch.manual_seed(0)
+    h, i, n = 64, 128, 8
+    r = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+    x, w = r(4, h), r(h)
+    mlp = [r(i, h), r(i, h), r(h, i)]
+    rest = [r(n, h), r(n, h), r(n * n, h), r(n * n, h)]
+    fold = [torch.ones(2 * n, device="cuda"), torch.zeros(2 * n, device="cuda")]
+    calls = [(lambda a: omni_rms_norm_func(a[0], a[1], a[2]), [x, w, x.clone()]),
+             (lambda a: omni_mlp_ckpt_func(*a), [x, *mlp]),
+             (lambda a: omni_decode_func(*a[:8], 4, *a[8:]), [x, *mlp, *rest, *fold])]
+    for call, args in calls:
+        call(args)
+        with fw.dual_level():
+            call(args)             # nothing carries a tangent
+            for j in range(len(args)):
+                dual = [fw.make_dual(a, torch.ones_like(a)) if q == j else a for q, a in enumerate(args)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(dual)
+                leaf = [a.clone().requires_grad_() if q != j and call is not calls[2][0] else a for q, a in enumerate(dual)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(leaf)
+        call(args)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: omni_rms_norm_func(v, w).y, (x,), (torch.ones_like(x),))
+    config = OmniMoEConfig(h, i, "silu", n * n, 4)
+    layer, block = OmniMoE(config).bfloat16().cuda().eval(), OmniMoEBlock(config).bfloat16().cuda().eval()
+    x = x[None]
+    for call in (layer.decode, block):
+        with fw.dual_level(), torch.no_grad():
+            call(x)
+        with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(fw.make_dual(x, torch.ones_like(x)))
+    weight = layer.gate_proj.weight
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.functional_call(Decoding(layer), {"layer.gate_proj.weight": fw.make_dual(weight.detach(), torch.ones_like(weight))}, (x,))
+
+
+class Decoding(torch.nn.Module):
+    def __init__(self, layer):
+        super().__init__()
+        self.layer = layer
+
+    def forward(self, x):
+        return self.layer.decode(x)
