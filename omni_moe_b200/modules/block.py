@@ -9,6 +9,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.nn.modules import module as nn_module
 
 from ..ops.norm import RmsNormOutput, omni_rms_norm_func
 from .omni_moe import OmniMoE, OmniMoEConfig
@@ -27,13 +28,21 @@ class RMSNorm(nn.Module):
         return omni_rms_norm_func(x, self.weight, residual, self.eps, quantize)
 
 
+def _calls_plain_forward(layer: nn.Module) -> bool:
+    """Whether ``layer(x)`` is ``OmniMoE.forward(layer, x)`` and nothing else: no hooks, of its own or of all modules, and nobody's
+    wrapper around it."""
+    return (isinstance(layer, OmniMoE) and type(layer).forward is OmniMoE.forward and "forward" not in layer.__dict__
+            and not (layer._forward_hooks or layer._forward_pre_hooks or nn_module._global_forward_hooks
+                     or nn_module._global_forward_pre_hooks))
+
+
 class OmniMoEBlock(nn.Module):
     """Residual addition, norm and layer: ``(y, h)`` from ``hidden_states`` and the residual stream so far, where ``h`` is the new
     residual stream and ``y`` what the next block adds to it.
 
-    In eval mode without gradients, up to 64 tokens run as two kernels (norm, :meth:`OmniMoE.decode`); otherwise the layer's
-    :meth:`OmniMoE.forward` follows the norm.  ``checkpoint_bits=8`` keeps the shared MLP's pre-activations in 8 bits for the
-    backward (:meth:`OmniMoE.checkpoint_activations`).
+    In eval mode without gradients, up to 64 tokens run as two kernels (norm, :meth:`OmniMoE.decode`); otherwise, and where hooks
+    or a wrapper of ``layer`` want to see the call, ``layer(y)`` follows the norm.  ``checkpoint_bits=8`` keeps the shared MLP's
+    pre-activations in 8 bits for the backward (:meth:`OmniMoE.checkpoint_activations`).
     """
 
     DECODE_TOKENS = 64
@@ -46,6 +55,7 @@ class OmniMoEBlock(nn.Module):
     def forward(self, hidden_states: torch.Tensor, residual: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
         out = self.norm(hidden_states, residual)
         tokens = hidden_states.shape[:-1].numel()
-        if not self.layer.training and not out.y.requires_grad and 0 < tokens <= self.DECODE_TOKENS:
+        if (0 < tokens <= self.DECODE_TOKENS and not self.layer.training and not out.y.requires_grad
+                and _calls_plain_forward(self.layer)):
             return self.layer.decode(out.y), out.h
         return self.layer(out.y), out.h

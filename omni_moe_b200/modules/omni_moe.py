@@ -97,7 +97,7 @@ class OmniMoE(nn.Module):
         self._bn_cache = None
         self._bn_pair = None
         self._checkpoint_bits = 16
-        self.last_routing = None  # (scores, indices, weights) of the latest forward, for inspection
+        self.last_routing = None  # (scores, indices, weights) of the latest forward, for inspection; None after decode()
 
     def checkpoint_activations(self, bits: int = 8) -> "OmniMoE":
         """What the shared MLP keeps of its gate | up pre-activations for the backward: 16 bits a value (bf16, the default) or
@@ -422,6 +422,7 @@ class OmniMoE(nn.Module):
             raise ValueError(f"hidden_states must be (batch, sequence, {self.hidden_size}), got {tuple(hidden_states.shape)}")
         y = omni_decode_func(hidden_states.reshape(-1, self.hidden_size), *operands, self.top_k, *self._bn_fold_decode())
         self.last_status = _lib.device_status(hidden_states.device)
+        self.last_routing = None
         return y.view(hidden_states.shape)
 
     def graphed(self, num_tokens: int, device=None) -> "GraphedOmniMoE":

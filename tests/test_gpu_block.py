@@ -176,3 +176,55 @@ class Decoding(torch.nn.Module):
 
     def forward(self, x):
         return self.layer.decode(x)
+
+
+def test_hooks_of_the_layer_run_whatever_the_number_of_tokens():
+    b, = [b.eval() for b in blocks(1)]
+    few, many = (torch.randn(1, t, 256, device="cuda").bfloat16() for t in (64, 65))
+    seen = []
+    with torch.no_grad():
+        for register in (lambda: b.layer.register_forward_hook(lambda m, a, y: seen.append(y.shape[1]) or 0 * y),
+                         lambda: b.layer.register_forward_pre_hook(lambda m, a: seen.append(a[0].shape[1]) or (0 * a[0],)),
+                         lambda: torch.nn.modules.module.register_module_forward_hook(
+                             lambda m, a, y: (seen.append(y.shape[1]) or 0 * y) if m is b.layer else None)):
+            handle = register()
+            seen.clear()
+            try:
+                outs = [b(x)[0] for x in (few, many)]
+            finally:
+                handle.remove()
+            assert seen == [64, 65] and not any(y.any() for y in outs)
+        seen.clear()
+        assert b(few)[0].any() and not seen
+
+
+def test_another_layer_in_the_block():
+    """A layer that is wrapped or replaced is called as it is."""
+    class Twice(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner = inner
+
+        def forward(self, x):
+            return 2 * self.inner(x)
+
+    b, = [b.eval() for b in blocks(1)]
+    x = torch.randn(1, 5, 256, device="cuda").bfloat16()
+    with torch.no_grad():
+        n = b.norm(x).y
+        want = 2 * b.layer(n)
+        b.layer = Twice(b.layer)
+        assert torch.equal(b(x)[0], want)
+        b.layer = b.layer.inner
+        forward = b.layer.forward
+        b.layer.forward = lambda v: 2 * forward(v)   # as wrappers of a module's forward do
+        assert torch.equal(b(x)[0], want)
+
+
+def test_no_routing_of_an_earlier_call_is_left():
+    b, = [b.eval() for b in blocks(1)]
+    with torch.no_grad():
+        b(torch.randn(1, 80, 256, device="cuda").bfloat16())
+        assert b.layer.last_routing[1].shape == (80, 8)
+        b(torch.randn(1, 5, 256, device="cuda").bfloat16())
+        assert b.layer.last_routing is None    # the one kernel keeps its selection to itself
