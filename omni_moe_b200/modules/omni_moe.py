@@ -126,16 +126,22 @@ class OmniMoE(nn.Module):
         scale = torch.rsqrt(var + eps)
         return scale.contiguous(), (-mean * scale).contiguous()
 
+    def _bn_fold_sources(self):
+        """What the fold is computed from: four tensors, and the numbers that change when their contents or storages do (held
+        with the tensors, as an address may come back with another tensor) or that enter the fold themselves."""
+        bx, by = self.router_norm_x, self.router_norm_y
+        tensors = (bx.running_mean, bx.running_var, by.running_mean, by.running_var)
+        return tensors, (bx.eps, by.eps, *(v for t in tensors for v in (t._version, t.data_ptr())))
+
     def _bn_fold_eval(self):
         """Eval-mode BatchNorm of both axes as one scale / shift pair per logit column."""
-        bx, by = self.router_norm_x, self.router_norm_y
-        key = (bx.running_mean._version, bx.running_var._version, by.running_mean._version, by.running_var._version,
-               bx.running_mean.data_ptr(), by.running_mean.data_ptr())
-        if self._bn_cache is None or self._bn_cache[0] != key:
+        tensors, numbers = self._bn_fold_sources()
+        kept = self._bn_cache
+        if kept is None or kept[0][1] != numbers or any(a is not b for a, b in zip(kept[0][0], tensors)):
             fold = self._bn_fold_values()
             if fold[0].is_cuda and torch.cuda.is_current_stream_capturing():
                 return fold  # the graph's own memory, computed in every replay: not to be kept
-            self._bn_cache = (key, *fold)
+            self._bn_cache = ((tensors, numbers), *fold)
         return self._bn_cache[1], self._bn_cache[2]
 
     def _bn_fold_decode(self):
