@@ -68,7 +68,47 @@ class _Buffers:
         self.ev_join = torch.cuda.Event()
 
 
+class _BatchNormFold:
+    """The kept scale / shift pair and what it was made from.
+
+    Eager calls may come on any stream: a stream other than the maker's waits for the pair once.  From then on, or once a capture
+    has taken the addresses (its graph may replay at any time on any stream), the pair keeps its memory, and new values are
+    written into it with the device idle.  A pair that one stream alone has read is replaced without waiting."""
+
+    def __init__(self, sources, scale: torch.Tensor, shift: torch.Tensor):
+        self.sources, self.scale, self.shift = sources, scale, shift
+        self.shared = False
+        if scale.is_cuda:
+            stream = torch.cuda.current_stream(scale.device)
+            self.index, self.streams, self.made = scale.get_device(), {stream.cuda_stream}, stream.record_event()
+
+    def __reduce__(self):
+        return type(None), ()  # copied and pickled modules make their own
+
+    def made_from(self, sources) -> bool:
+        return self.sources is not None and self.sources[1] == sources[1] and all(a is b for a, b in zip(self.sources[0], sources[0]))
+
+    def pair(self):
+        if self.scale.is_cuda:
+            stream = _lib.stream_ptr(self.index)
+            if torch.cuda.is_current_stream_capturing():
+                self.shared = True
+            elif stream not in self.streams:
+                torch.cuda.current_stream(self.index).wait_event(self.made)
+                self.streams.add(stream)
+                self.shared = True
+        return self.scale, self.shift
+
+    def overwrite(self, sources, scale: torch.Tensor, shift: torch.Tensor) -> None:
+        torch.cuda.synchronize(self.index)  # nothing in flight reads the old values any more
+        self.scale.copy_(scale), self.shift.copy_(shift)
+        torch.cuda.current_stream(self.index).synchronize()  # and everything issued from here on reads the new ones
+        self.sources = sources
+
+
 class OmniMoE(nn.Module):
+    _bn_fold = None  # _BatchNormFold of the running statistics
+
     def __init__(self, config: OmniMoEConfig):
         super().__init__()
         if config.hidden_act not in ("silu", "swish"):
@@ -94,8 +134,6 @@ class OmniMoE(nn.Module):
         self.down_embed = nn.Embedding(self.num_experts, self.hidden_size)
 
         self._buffers_cache: dict = {}
-        self._bn_cache = None
-        self._bn_pair = None
         self._checkpoint_bits = 16
         self.last_routing = None  # (scores, indices, weights) of the latest forward, for inspection; None after decode()
 
@@ -134,36 +172,19 @@ class OmniMoE(nn.Module):
         return tensors, (bx.eps, by.eps, *(v for t in tensors for v in (t._version, t.data_ptr())))
 
     def _bn_fold_eval(self):
-        """Eval-mode BatchNorm of both axes as one scale / shift pair per logit column."""
-        tensors, numbers = self._bn_fold_sources()
-        kept = self._bn_cache
-        if kept is None or kept[0][1] != numbers or any(a is not b for a, b in zip(kept[0][0], tensors)):
-            fold = self._bn_fold_values()
-            if fold[0].is_cuda and torch.cuda.is_current_stream_capturing():
-                return fold  # the graph's own memory, computed in every replay: not to be kept
-            self._bn_cache = ((tensors, numbers), *fold)
-        return self._bn_cache[1], self._bn_cache[2]
-
-    def _bn_fold_decode(self):
-        """The same pair for :meth:`decode`, at an address that stays (graphs may hold it) and ready for calls on any stream."""
-        scale, shift = self._bn_fold_eval()
-        pair = getattr(self, "_bn_pair", None)  # (the tensor it was copied from, scale, shift)
-        if pair is not None and pair[0] is scale:
-            return pair[1], pair[2]
-        if torch.cuda.is_current_stream_capturing():
-            kept = self._bn_cache is not None and self._bn_cache[1] is scale
-            return self._bn_fold_values() if kept else (scale, shift)  # part of the graph
-        with torch.no_grad(), torch.inference_mode(False):  # ordinary tensors, whoever asks first
-            # once per change of the statistics: no launch on any stream still reads the old values afterwards, and every
-            # stream may read the new ones
-            torch.cuda.synchronize(scale.device)
-            if pair is not None and pair[1].device == scale.device and pair[1].shape == scale.shape:
-                pair[1].copy_(scale), pair[2].copy_(shift)
-                self._bn_pair = (scale, pair[1], pair[2])
-            else:
-                self._bn_pair = (scale, scale.clone(), shift.clone())
-            torch.cuda.synchronize(scale.device)
-        return self._bn_pair[1], self._bn_pair[2]
+        """Eval-mode BatchNorm of both axes as one scale / shift pair per logit column, ready for the current stream."""
+        sources = self._bn_fold_sources()
+        fold = self._bn_fold
+        if fold is None or not fold.made_from(sources):
+            if sources[0][0].is_cuda and torch.cuda.is_current_stream_capturing():
+                return self._bn_fold_values()  # part of the graph, computed in every replay: not to be kept
+            with torch.no_grad(), torch.inference_mode(False):  # ordinary tensors, whoever asks first
+                scale, shift = self._bn_fold_values()
+                if fold is not None and fold.shared and fold.scale.device == scale.device and fold.scale.shape == scale.shape:
+                    fold.overwrite(sources, scale, shift)
+                else:
+                    fold = self._bn_fold = _BatchNormFold(sources, scale, shift)
+        return fold.pair()
 
     def sync_batch_statistics(self, group=None, enabled: bool = True) -> "OmniMoE":
         """Training-mode BatchNorm over the tokens of every rank of ``group`` (default: all ranks), for
@@ -201,7 +222,8 @@ class OmniMoE(nn.Module):
                 ptr(bx.running_mean), ptr(bx.running_var), ptr(by.running_mean), ptr(by.running_var), _lib.dtype_code(run_dt),
                 ptr(bx.num_batches_tracked), ptr(by.num_batches_tracked), b.bn_scale.data_ptr(), b.bn_shift.data_ptr(),
                 b.bn_scratch.data_ptr(), b.bn_scratch.numel(), _lib.stream_ptr()))
-            self._bn_cache = None  # the running statistics changed behind torch's version counters
+            if self._bn_fold is not None:
+                self._bn_fold.sources = None  # the running statistics changed behind torch's version counters
             return b.bn_scale, b.bn_shift
         if grp is None:
             t = logits.size(0)
@@ -261,6 +283,7 @@ class OmniMoE(nn.Module):
         main = torch.cuda.current_stream()
         st = main.cuda_stream
         status = b.status.data_ptr()
+        fold = None if self.training else self._bn_fold_eval()
         # 1. gate/up projections + SwiGLU: fills every SM
         chk(lib.omni_mlp_gate_up(x.data_ptr(), wg.data_ptr(), wu.data_ptr(), t, h, i, b.act.data_ptr(), status, st))
         b.ev_fork.record(main)
@@ -270,7 +293,7 @@ class OmniMoE(nn.Module):
             b.side.wait_event(b.ev_fork)
             ss = b.side.cuda_stream
             chk(lib.omni_router_gate(x.data_ptr(), kx.data_ptr(), ky.data_ptr(), t, h, n, b.logits.data_ptr(), status, ss))
-            scale, shift = self._bn_fold_train(b.logits, b) if self.training else self._bn_fold_eval()
+            scale, shift = fold if fold is not None else self._bn_fold_train(b.logits, b)
             if not routed:
                 chk(lib.omni_router_logits_topk(b.logits.data_ptr(), 2 * n, scale.data_ptr(), shift.data_ptr(), t, n, k,
                                                 b.scores.data_ptr(), b.indices.data_ptr(), 0, b.weights.data_ptr(),
@@ -426,7 +449,7 @@ class OmniMoE(nn.Module):
         operands = self._operands()
         if hidden_states.dim() != 3 or hidden_states.size(2) != self.hidden_size:
             raise ValueError(f"hidden_states must be (batch, sequence, {self.hidden_size}), got {tuple(hidden_states.shape)}")
-        y = omni_decode_func(hidden_states.reshape(-1, self.hidden_size), *operands, self.top_k, *self._bn_fold_decode())
+        y = omni_decode_func(hidden_states.reshape(-1, self.hidden_size), *operands, self.top_k, *self._bn_fold_eval())
         self.last_status = _lib.device_status(hidden_states.device)
         self.last_routing = None
         return y.view(hidden_states.shape)
@@ -465,8 +488,8 @@ class GraphedOmniMoE:
         self.buffers = _Buffers(num_tokens, module.hidden_size, module.intermediate_size, module.num_expert_sqrt,
                                 module.num_experts, module.top_k, dev)
         with torch.cuda.device(dev):
-            if not module.training:
-                module._bn_fold_eval()
+            # an eval-mode graph reads the module's BatchNorm fold: held here, brought up to date before every replay
+            self.fold = None if module.training else module._bn_fold_eval()
             # the warm-up launch of a training-mode module would count as a batch: keep the statistics as they were
             stats = [(buf, buf.clone()) for bn in (module.router_norm_x, module.router_norm_y)
                      for buf in (bn.running_mean, bn.running_var, bn.num_batches_tracked) if module.training and buf is not None]
@@ -484,10 +507,11 @@ class GraphedOmniMoE:
                 module._launch(self.x, self.y, self.buffers)
 
     def replay(self) -> torch.Tensor:
+        if self.fold is not None:
+            self.module._bn_fold_eval()
         self.graph.replay()
         return self.y
 
     def __call__(self, hidden_states: torch.Tensor) -> torch.Tensor:
         self.x.copy_(hidden_states.reshape(self.x.shape), non_blocking=True)
-        self.graph.replay()
-        return self.y.view(hidden_states.shape)
+        return self.replay().view(hidden_states.shape)
