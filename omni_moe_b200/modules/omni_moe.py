@@ -77,7 +77,7 @@ class _BatchNormFold:
 
     def __init__(self, sources, scale: torch.Tensor, shift: torch.Tensor):
         self.sources, self.scale, self.shift = sources, scale, shift
-        self.shared = False
+        self.shared = self.captured = False
         if scale.is_cuda:
             stream = torch.cuda.current_stream(scale.device)
             self.index, self.streams, self.made = scale.get_device(), {stream.cuda_stream}, stream.record_event()
@@ -92,7 +92,7 @@ class _BatchNormFold:
         if self.scale.is_cuda:
             stream = _lib.stream_ptr(self.index)
             if torch.cuda.is_current_stream_capturing():
-                self.shared = True
+                self.shared = self.captured = True
             elif stream not in self.streams:
                 torch.cuda.current_stream(self.index).wait_event(self.made)
                 self.streams.add(stream)
@@ -108,6 +108,7 @@ class _BatchNormFold:
 
 class OmniMoE(nn.Module):
     _bn_fold = None  # _BatchNormFold of the running statistics
+    _bn_moved_by_graphs = False  # whether a training forward was captured: its replays move the statistics unseen
 
     def __init__(self, config: OmniMoEConfig):
         super().__init__()
@@ -175,9 +176,11 @@ class OmniMoE(nn.Module):
         """Eval-mode BatchNorm of both axes as one scale / shift pair per logit column, ready for the current stream."""
         sources = self._bn_fold_sources()
         fold = self._bn_fold
-        if fold is None or not fold.made_from(sources):
+        if self._bn_moved_by_graphs or fold is None or not fold.made_from(sources):
             if sources[0][0].is_cuda and torch.cuda.is_current_stream_capturing():
                 return self._bn_fold_values()  # part of the graph, computed in every replay: not to be kept
+            if self._bn_moved_by_graphs and (fold is None or not fold.captured):
+                return self._bn_fold_values()  # may be old by the next call
             with torch.no_grad(), torch.inference_mode(False):  # ordinary tensors, whoever asks first
                 scale, shift = self._bn_fold_values()
                 if fold is not None and fold.shared and fold.scale.device == scale.device and fold.scale.shape == scale.shape:
@@ -202,12 +205,17 @@ class OmniMoE(nn.Module):
             return (self.router_norm_x.process_group,)
         return None
 
+    def _note_captured_step(self) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            self._bn_moved_by_graphs = True
+
     def _bn_fold_train(self, logits: torch.Tensor, b: "_Buffers | None" = None):
         """Training-mode BatchNorm: batch statistics over all tokens (of all ranks, when synchronised),
         running statistics updated as nn.BatchNorm1d does (momentum average, unbiased variance).
         On one rank this is the library's kernel pair (no allocation, no host read: capturable); with
         synchronised statistics the per-rank moments are merged through torch.distributed."""
         n = self.num_expert_sqrt
+        self._note_captured_step()
         grp = self._bn_group()
         bx, by = self.router_norm_x, self.router_norm_y
         run_dt = bx.running_mean.dtype if bx.running_mean is not None else torch.float32
@@ -393,6 +401,8 @@ class OmniMoE(nn.Module):
             scores, indices = RouterFrontFunction.apply(x, self.router_gate_x.weight, self.router_gate_y.weight, self.top_k,
                                                         fold, self.training)
         else:
+            if self.training:
+                self._note_captured_step()
             logits_x = self.router_norm_x(self.router_gate_x(x))
             logits_y = self.router_norm_y(self.router_gate_y(x))
             # log-probabilities, scores and routing weights stay in fp32 (the reference keeps the module dtype):
@@ -488,8 +498,9 @@ class GraphedOmniMoE:
         self.buffers = _Buffers(num_tokens, module.hidden_size, module.intermediate_size, module.num_expert_sqrt,
                                 module.num_experts, module.top_k, dev)
         with torch.cuda.device(dev):
-            # an eval-mode graph reads the module's BatchNorm fold: held here, brought up to date before every replay
-            self.fold = None if module.training else module._bn_fold_eval()
+            # an eval-mode graph reads the module's BatchNorm fold (held here, brought up to date before every replay) or makes
+            # its own
+            self.fold = None if module.training or module._bn_moved_by_graphs else module._bn_fold_eval()
             # the warm-up launch of a training-mode module would count as a batch: keep the statistics as they were
             stats = [(buf, buf.clone()) for bn in (module.router_norm_x, module.router_norm_y)
                      for buf in (bn.running_mean, bn.running_var, bn.num_batches_tracked) if module.training and buf is not None]

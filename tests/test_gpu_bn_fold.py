@@ -132,3 +132,47 @@ def test_one_stream_does_not_wait():
         m.decode(x), m(x)
         assert not done.query()
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("how", ["graphed", "raw"])
+def test_statistics_that_a_captured_training_step_moves(how):
+    """Replays move the running statistics without any Python code: eval calls between them see each step's."""
+    m, x = layer()
+    m.train()
+    if how == "graphed":
+        g = m.graphed(96)
+        step = lambda: g(x)
+    else:
+        # a step through the differentiable form, as a training program captures it
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            torch.autograd.grad(m(x).float().square().mean(), m.gate_proj.weight)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(m(x).float().square().mean(), m.gate_proj.weight)
+        step = graph.replay
+    m.eval()
+    outs = []
+    with torch.no_grad():
+        for _ in range(3):
+            step()
+            want = fresh(m, x)
+            assert torch.equal(m(x), want)
+            few = fresh(m, x[:, :7]), m.decode(x[:, :7])
+            assert float((few[1].double() - few[0].double()).norm() / few[0].double().norm()) < 2 ** -7
+            other, _ = layer()
+            other.load_state_dict(m.state_dict())
+            assert torch.equal(few[1], other.eval().decode(x[:, :7]))
+            outs.append(want)
+    assert not torch.equal(outs[0], outs[2])
+
+
+def test_eval_graph_beside_a_training_graph():
+    m, x = layer()
+    trained, tested = m.train().graphed(96), m.eval().graphed(96)
+    with torch.no_grad():
+        for _ in range(2):
+            trained(x)
+            assert torch.equal(tested(x), fresh(m, x))
