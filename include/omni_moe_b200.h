@@ -529,13 +529,14 @@ OMNI_API int omni_router_norm_bwd(const float *dscores, const int32_t *indices, 
  *   [num_experts, H]  bf16, row-major, 16-byte aligned;  H (<= 16384) and I multiples of 8
  *   bn_scale, bn_shift [2*sqrt_n] fp32: normalised = logit * scale + shift (both NULL = identity)
  *   y [T, H] bf16, may not overlap any input
- *   workspace: omni_decode_workspace_bytes(...) bytes, 16-byte aligned, whose first 8704 bytes were zero before the
- *   first launch that uses it; every launch leaves them zero.  Launches that may overlap on the GPU (other streams,
+ *   workspace: omni_decode_workspace_bytes(...) bytes, 16-byte aligned, whose first omni_decode_counter_bytes()
+ *   were zero before the first launch that uses it; every launch leaves them zero and writes the rest before it reads it.  Launches that may overlap on the GPU (other streams,
  *   captured graphs that replay beside each other) need a workspace each.
  * The kernel is launched cooperatively (its blocks wait on one another; each wait is bounded and sets
  * OMNI_ST_WAIT_TIMEOUT).  Run-to-run identical: no atomics on results.
  */
 OMNI_API int omni_decode_max_tokens(void);
+OMNI_API size_t omni_decode_counter_bytes(void);
 OMNI_API size_t omni_decode_workspace_bytes(int num_tokens, int hidden, int intermediate, int sqrt_n, int k);
 OMNI_API int omni_decode(const void *x, const void *gate_w, const void *up_w, const void *down_w, const void *router_x,
                          const void *router_y, const void *up_table, const void *down_table, const float *bn_scale,

@@ -103,6 +103,7 @@ SIGNATURES = {
     "omni_mlp_dact_swiglu_mx": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
                                         c_void_p, c_void_p]),
     "omni_decode_max_tokens": (c_int, []),
+    "omni_decode_counter_bytes": (c_size_t, []),
     "omni_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "omni_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),

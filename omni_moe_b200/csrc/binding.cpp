@@ -319,11 +319,15 @@ Tensor mlp_ckpt(const Tensor& x, const Tensor& gate, const Tensor& up, const Ten
 // ---- the layer for a few tokens -------------------------------------------------------------------
 // Scratch of a call on the current stream; its head holds counters that every launch finds and leaves at zero.  One
 // buffer for each (device, stream): launches on one stream follow one another, launches on different streams may overlap
-// and must not share.  While a graph is captured the buffer belongs to the graph (zeroed in every replay), so graphs that
+// and must not share.  While a graph is captured the buffer belongs to the graph (its head zeroed in every replay), so graphs that
 // replay beside each other or beside eager calls share nothing.
 Tensor decode_workspace(int64_t bytes, const Tensor& like, void* stream) {
-  const auto bytes_of = like.options().dtype(at::kByte);
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return at::zeros({bytes}, bytes_of);
+  const auto fresh = [&] {
+    Tensor ws = at::empty({bytes}, like.options().dtype(at::kByte));
+    ws.narrow(0, 0, static_cast<int64_t>(omni_decode_counter_bytes())).zero_();
+    return ws;
+  };
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return fresh();
   static std::mutex mutex;
   static auto* buffers = new std::map<std::pair<int, void*>, Tensor>();  // never destroyed: CUDA may be gone by then
   const std::lock_guard<std::mutex> lock(mutex);
@@ -333,7 +337,7 @@ Tensor decode_workspace(int64_t bytes, const Tensor& like, void* stream) {
   // a buffer that is dropped goes back to its own stream's pool: launches in flight keep it
   if (it != buffers->end()) buffers->erase(it);
   while (buffers->size() >= 16) buffers->erase(buffers->begin());
-  return buffers->emplace(key, at::zeros({bytes}, bytes_of)).first->second;
+  return buffers->emplace(key, fresh()).first->second;
 }
 
 // Nothing where something has to be converted, copied or padded first.

@@ -1211,6 +1211,8 @@ using namespace omni;
 
 extern "C" int omni_decode_max_tokens(void) { return kDecMaxTokens; }
 
+extern "C" size_t omni_decode_counter_bytes(void) { return CNT_WORDS * 4; }
+
 extern "C" size_t omni_decode_workspace_bytes(int num_tokens, int hidden, int intermediate, int sqrt_n, int k) {
   if (num_tokens < 1 || num_tokens > kDecMaxTokens || hidden < 8 || intermediate < 8 || sqrt_n < 1 || k < 1) return 0;
   const int64_t T = num_tokens;

@@ -403,3 +403,24 @@ def test_weights_that_require_gradients_are_refused():
     odd = make(3, 60, 64, 8, 4, 1)   # sizes that are padded first
     with pytest.raises(RuntimeError, match="no backward"):
         call(odd, wg=odd["wg"].clone().requires_grad_())
+
+
+@pytest.mark.parametrize("t,h,i,n,k", [(3, 256, 1024, 32, 8), (14, 512, 1024, 64, 16), (24, 512, 2048, 64, 16), (64, 1024, 512, 200, 40),
+                                       (18, 8, 8, 3, 2), (16, 4096, 8192, 30, 16)])
+def test_workspace_of_the_c_entry(t, h, i, n, k):
+    """Only the counters at its head need to be zero: whatever else is there is written before it is read."""
+    from omni_moe_b200 import _lib
+    lib = _lib.load()
+    p = make(t, h, i, n, k, 3, table_std=0.1)
+    head, size = lib.omni_decode_counter_bytes(), lib.omni_decode_workspace_bytes(t, h, i, n, k)
+    assert 0 < head < size and head % 16 == 0
+    ws = torch.full((size + 64,), 0xff, device="cuda", dtype=torch.uint8)   # NaN in fp32 and bf16
+    ws[:head] = 0
+    for _ in range(2):
+        y = torch.empty_like(p["x"])
+        _lib.check(lib.omni_decode(*(p[a].data_ptr() for a in ("x", "wg", "wu", "wd", "kx", "ky", "up", "down", "scale", "shift")), t, h, i, n, k,
+                                   n * n, y.data_ptr(), ws.data_ptr(), size, _lib.device_status("cuda").data_ptr(), _lib.stream_ptr()))
+        _lib.check_device_status()
+        assert torch.equal(y, call(p))
+        assert not ws[:head].any() and (ws[size:] == 0xff).all()
+        ws[head:size] = 0xff
