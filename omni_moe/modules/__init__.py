@@ -1,1 +1,1 @@
-from omni_moe_b200.modules.omni_moe import OmniMoE, OmniMoEConfig  # noqa: F401
+from omni_moe_b200.modules import OmniMoE, OmniMoEBlock, OmniMoEConfig, RMSNorm  # noqa: F401

@@ -81,3 +81,14 @@ def test_forward_mode_is_seen_before_anything_runs():
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
         with fw.dual_level(), pytest.raises(RuntimeError, match="CUDA tensors only"):
             call(x)
+
+
+def test_names_under_the_reference_paths():
+    """What stands beside the layer is found where the layer is, under either package."""
+    import omni_moe.modules
+    import omni_moe.ops
+    import omni_moe_b200.modules
+    import omni_moe_b200.ops
+    for ours, theirs in ((omni_moe_b200.modules, omni_moe.modules), (omni_moe_b200.ops, omni_moe.ops)):
+        for name in ours.__all__:
+            assert getattr(theirs, name) is getattr(ours, name)
