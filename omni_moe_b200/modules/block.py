@@ -54,8 +54,7 @@ class OmniMoEBlock(nn.Module):
 
     def forward(self, hidden_states: torch.Tensor, residual: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
         out = self.norm(hidden_states, residual)
-        tokens = hidden_states.shape[:-1].numel()
-        if (0 < tokens <= self.DECODE_TOKENS and not self.layer.training and not out.y.requires_grad
-                and _calls_plain_forward(self.layer)):
-            return self.layer.decode(out.y), out.h
-        return self.layer(out.y), out.h
+        layer, tokens = self.layer, hidden_states.shape[:-1].numel()
+        if 0 < tokens <= self.DECODE_TOKENS and not layer.training and not out.y.requires_grad and _calls_plain_forward(layer):
+            return layer.decode(out.y), out.h
+        return layer(out.y), out.h

@@ -23,6 +23,7 @@ import torch
 import torch.nn as nn
 
 from .. import _lib
+from ..ops._common import in_dual_level, refuse_tangents
 from ..ops.expert import hot_workspace, use_fused_path, use_hot_experts, use_routed_kernel
 from ..ops.scheduler import workspace_bytes
 
@@ -78,7 +79,8 @@ class _BatchNormFold:
     def __init__(self, sources, scale: torch.Tensor, shift: torch.Tensor):
         self.sources, self.scale, self.shift = sources, scale, shift
         self.shared = self.captured = False
-        if scale.is_cuda:
+        self.cuda = scale.is_cuda
+        if self.cuda:
             stream = torch.cuda.current_stream(scale.device)
             self.index, self.streams, self.made = scale.get_device(), {stream.cuda_stream}, stream.record_event()
 
@@ -86,10 +88,10 @@ class _BatchNormFold:
         return type(None), ()  # copied and pickled modules make their own
 
     def made_from(self, sources) -> bool:
-        return self.sources is not None and self.sources[1] == sources[1] and all(a is b for a, b in zip(self.sources[0], sources[0]))
+        return self.sources is not None and self.sources[1] == sources[1]
 
     def pair(self):
-        if self.scale.is_cuda:
+        if self.cuda:
             stream = _lib.stream_ptr(self.index)
             if torch.cuda.is_current_stream_capturing():
                 self.shared = self.captured = True
@@ -166,11 +168,12 @@ class OmniMoE(nn.Module):
         return scale.contiguous(), (-mean * scale).contiguous()
 
     def _bn_fold_sources(self):
-        """What the fold is computed from: four tensors, and the numbers that change when their contents or storages do (held
-        with the tensors, as an address may come back with another tensor) or that enter the fold themselves."""
+        """What the fold is computed from: four tensors, and a key that changes when one of them, its contents or its storage
+        does, or an eps (kept beside the tensors themselves, so that no id comes back with another tensor)."""
         bx, by = self.router_norm_x, self.router_norm_y
-        tensors = (bx.running_mean, bx.running_var, by.running_mean, by.running_var)
-        return tensors, (bx.eps, by.eps, *(v for t in tensors for v in (t._version, t.data_ptr())))
+        a, b, c, d = tensors = bx.running_mean, bx.running_var, by.running_mean, by.running_var
+        return tensors, (bx.eps, by.eps, id(a), id(b), id(c), id(d), a._version, b._version, c._version, d._version,
+                         a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr())
 
     def _bn_fold_eval(self):
         """Eval-mode BatchNorm of both axes as one scale / shift pair per logit column, ready for the current stream."""
@@ -449,7 +452,6 @@ class OmniMoE(nn.Module):
         only its output (and a per-stream workspace once), so it can be captured in a CUDA graph, best after one call
         outside it (the BatchNorm fold of the running statistics is then not part of the graph, and replays see the
         statistics of the module's latest call); inference only."""
-        from ..ops._common import in_dual_level, refuse_tangents
         from ..ops.decode import omni_decode_func
         if self.training:
             raise RuntimeError("decode() uses the running statistics of the router's BatchNorm: call eval() first")
@@ -461,7 +463,8 @@ class OmniMoE(nn.Module):
             raise ValueError(f"hidden_states must be (batch, sequence, {self.hidden_size}), got {tuple(hidden_states.shape)}")
         y = omni_decode_func(hidden_states.reshape(-1, self.hidden_size), *operands, self.top_k, *self._bn_fold_eval())
         self.last_status = _lib.device_status(hidden_states.device)
-        self.last_routing = None
+        if self.last_routing is not None:
+            self.last_routing = None
         return y.view(hidden_states.shape)
 
     def graphed(self, num_tokens: int, device=None) -> "GraphedOmniMoE":

@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._common import aligned, as_bf16, pad_both, pad_last, refuse_tangents
+from ._common import aligned, as_bf16, in_dual_level, pad_both, pad_last, refuse_tangents
 
 
 def omni_decode_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, down_weight: torch.Tensor,
@@ -28,7 +28,8 @@ def omni_decode_func(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
     Operands are bf16 (others are rounded to it per call), sums fp32.  Inference only: with gradients enabled, a call with a
     tensor that requires them is refused.  Device-side faults are reported by ``check_device_status``.
     """
-    refuse_tangents("omni_decode_func", x, gate_weight, up_weight, down_weight, router_x, router_y, up_embed, down_embed, bn_scale, bn_shift)
+    if in_dual_level():
+        refuse_tangents("omni_decode_func", x, gate_weight, up_weight, down_weight, router_x, router_y, up_embed, down_embed, bn_scale, bn_shift)
     k = int(num_experts_per_token)
     y = _lib.binding().decode(x, gate_weight, up_weight, down_weight, router_x, router_y, up_embed, down_embed, k, bn_scale, bn_shift,
                               _lib.status_ptr(x))
