@@ -341,3 +341,31 @@ def test_scale_that_is_no_number(i, limit):
     for got, was, nan, same in zip(start(bad), clean, (gate | (up & within[0]), gate & within[1], gate | up), (torch.ones_like(cut), ~cut, torch.ones_like(cut))):
         assert torch.isfinite(was).all()
         assert got[nan].isnan().all() and torch.isfinite(got[~nan]).all() and torch.equal(got[~nan & same], was[~nan & same])
+
+
+@pytest.mark.parametrize("t,h,i", [(77, 256, 1024), (256, 512, 64), (515, 1000, 2760), (1024, 1024, 4096)])
+def test_gradients_round_twice(t, h, i):
+    """The activation's gradient stays in fp32 on its way to dgate | dup: a gradient has two roundings to bf16 in it, that of
+    dgate | dup (or of the activation) and its own.  Each is at most R of the value, so R of the result and 1.01 R (R, and R of
+    R again) of the sum of magnitudes.  In the mean square a rounding is R / sqrt(3) of the value at the start of an octave and
+    half of that at its end: 0.425 R over values that spread like sums and products of normal ones, 0.60 R for two and 0.74 R
+    for three; between them, 0.66 R is asked for."""
+    from omni_moe_b200.ops import mx_dequantize, mx_quantize
+    from omni_moe_b200.ops.mlp_ckpt import mlp_ckpt_backward
+    (x, wg, wu, wd), dy = make(t, h, i, t + h)
+    _, codes, scales = forward(x, wg, wu)
+    xq = mx_dequantize(*mx_quantize(x))
+    got = mlp_ckpt_backward(dy, xq, codes, scales, wg, wu, wd)
+    g, u = decoded(codes, scales)
+    act, sg, su = derivative(g, u, 0.0)
+    d = [v.double() for v in (dy, xq, wg, wu, wd)]
+    dact, amag = d[0] @ d[4], d[0].abs() @ d[4].abs()
+    dg, du, mg, mu = dact * sg, dact * su, amag * sg.abs(), amag * su.abs()
+    for a, ref, rounded, terms in (
+            (got[0], dg @ d[2] + du @ d[3], dg.abs() @ d[2].abs() + du.abs() @ d[3].abs(), mg @ d[2].abs() + mu @ d[3].abs()),
+            (got[1], dg.t() @ d[1], dg.abs().t() @ d[1].abs(), mg.t() @ d[1].abs()),
+            (got[2], du.t() @ d[1], du.abs().t() @ d[1].abs(), mu.t() @ d[1].abs()),
+            (got[3], d[0].t() @ act, d[0].abs().t() @ act.abs(), d[0].abs().t() @ act.abs())):
+        off = (a.double() - ref).abs()
+        assert (off <= R * ref.abs() + 1.01 * R * rounded + 1e-5 * terms + 1e-9).all()
+        assert float(off.norm() / ref.norm()) < 0.66 * R

@@ -405,3 +405,36 @@ def test_every_scale_byte(cols, dtype):
     want = (value * scale).to(dtype)
     assert torch.equal(got.isnan(), (byte == 255).repeat_interleave(32, 1)[:, :cols])
     assert torch.equal(got.nan_to_num(nan=0.0, posinf=float("inf")), want.nan_to_num(nan=0.0, posinf=float("inf")))
+
+
+def weight_sum_depth(t, n, dtype):
+    """Roundings that a term of the weight's gradient goes through, from the launch's shape: rows of a block in turn, the block's
+    row groups, every 32nd block's partial row in turn, and a tree over 32 of those sums."""
+    ve = 128 // torch.finfo(dtype).bits
+    per = 16 if n % ve == 0 and t >= 1024 else 8
+    while 512 * per < n:
+        per *= 2
+    warps = -(-n // (32 * per))
+    rpc = min(t, 8 // warps or 1)
+    threads, turns, sms = 32 * warps * rpc, -(-t // rpc), torch.cuda.get_device_properties(0).multi_processor_count
+    most = (3 if threads < 256 else max(1, 768 // threads)) * sms
+    blocks = min(most, min(turns, sms) if turns // 4 < sms else turns // 4)
+    return -(-turns // blocks) + rpc + -(-blocks // 32) + 5, blocks
+
+
+@pytest.mark.parametrize("t,n,dtype", [(16384, 4096, torch.bfloat16), (16384, 1024, torch.float32), (30001, 136, torch.float16),
+                                       (5000, 8192, torch.bfloat16), (20000, 70, torch.bfloat16), (100000, 256, torch.bfloat16), (1, 40, torch.float32)])
+def test_weight_gradient_of_many_rows(t, n, dtype):
+    from omni_moe_b200.ops import omni_rms_norm_func
+    g = torch.Generator("cuda").manual_seed(t + n)
+    x, dy, w = (torch.randn(*s, generator=g, device="cuda").to(dtype) for s in ((t, n), (t, n), (n,)))
+    w.requires_grad_()
+    dw, = torch.autograd.grad(omni_rms_norm_func(x, w, eps=1e-5).y, w, dy)
+    depth, blocks = weight_sum_depth(t, n, dtype)
+    if (t, n) == (16384, 4096):
+        assert blocks == 3 * torch.cuda.get_device_properties(0).multi_processor_count  # every block there is, 37 rows in turn
+    h = x.double()
+    terms = dy.double() * (h / torch.sqrt(h.square().mean(1, True) + 1e-5))
+    ref = terms.sum(0)
+    tol = half_step(dtype) * ref.abs() + (F + depth * 2 ** -24) * terms.abs().sum(0) * (1 + half_step(dtype)) + 2 ** -25
+    assert ((dw.double() - ref).abs() <= tol).all()
