@@ -21,7 +21,6 @@ using OptTensor = std::optional<Tensor>;
 
 constexpr int64_t kBlock = 32;          // values that share a scale
 constexpr int64_t kMaxHidden = 16384;   // of the norm
-constexpr int64_t kMaxDecodeTokens = 64;
 
 // ValueError / TypeError of the wrong argument
 #define OMNI_VALUE(cond, ...) \
@@ -352,7 +351,7 @@ OptTensor decode(const Tensor& x, const Tensor& gate, const Tensor& up, const Te
   }
   const int64_t t = x.size(0), h = x.size(1), i = gate.size(0), n = router_x.size(0), experts = up_embed.size(0);
   const auto is = [](const Tensor& m, int64_t r, int64_t c) { return m.size(0) == r && m.size(1) == c; };
-  OMNI_VALUE(t <= kMaxDecodeTokens, "omni_decode_func takes at most ", kMaxDecodeTokens, " tokens, got ", t, ": use OmniMoE.forward");
+  OMNI_VALUE(t <= omni_decode_max_tokens(), "omni_decode_func takes at most ", omni_decode_max_tokens(), " tokens, got ", t, ": use OmniMoE.forward");
   OMNI_VALUE(is(gate, i, h) && is(up, i, h) && is(down, h, i),
                     "gate_weight and up_weight must be (intermediate, hidden), down_weight (hidden, intermediate)");
   OMNI_VALUE(is(router_x, n, h) && is(router_y, n, h), "router_x and router_y must both be (sqrt_n, hidden)");

@@ -45,6 +45,9 @@ class OmniMoEBlock(nn.Module):
     pre-activations in 8 bits for the backward (:meth:`OmniMoE.checkpoint_activations`).
     """
 
+    # All that decode() takes: it is the faster at every number of tokens.  Device time, cold L2, decode / forward in us at 1, 16
+    # and 64 tokens: 256 x 1024 16 / 35, 17 / 34, 23 / 34; 1024 x 4096 21 / 115, 23 / 61, 30 / 61; 2048 x 8192 34 / 139, 41 / 141,
+    # 47 / 145; 4096 x 11008 with 64 of 2^20 experts 64 / 230, 78 / 226, 90 / 228.
     DECODE_TOKENS = 64
 
     def __init__(self, config: OmniMoEConfig, eps: float = 1e-6, checkpoint_bits: int = 16):

@@ -92,3 +92,9 @@ def test_names_under_the_reference_paths():
     for ours, theirs in ((omni_moe_b200.modules, omni_moe.modules), (omni_moe_b200.ops, omni_moe.ops)):
         for name in ours.__all__:
             assert getattr(theirs, name) is getattr(ours, name)
+
+
+def test_the_block_asks_for_no_more_tokens_than_the_kernel_takes():
+    from omni_moe_b200 import _lib
+    from omni_moe_b200.modules import OmniMoEBlock
+    assert OmniMoEBlock.DECODE_TOKENS <= _lib.load().omni_decode_max_tokens()
