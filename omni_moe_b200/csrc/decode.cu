@@ -20,7 +20,8 @@
 // Measured (B200, CUDA graph; floor = bytes at 6547 GB/s): 1 token x 256 x 1024 12.2 us (latency: five dependent passes
 // through L2 and a cooperative launch), 1 x 1024 x 4096 15.8 us (floor 3.9), 8 x 4096 x 11008 56.5 us (42.6: 75 % of the
 // copy rate), 64 x 2048 x 8192 40.4 us (17.1), 24 x 4096 x 11008 with 64 of 2^20 experts 69.5 us (47.8).
-// The layer's four-kernel forward takes as long for one token as for 256.
+// The layer's four-kernel forward takes 34 us for 1 to 64 tokens of 256 x 1024, where this takes 16 to 23, and 141 us for
+// 2048 x 8192, where this takes 34 to 47 (events around one call, cold L2).
 //
 // act is rounded to bf16 (it is an operand of the down projection); everything else is summed in fp32 and y is rounded
 // once.
@@ -1153,7 +1154,7 @@ template <int N>
 int launch_ring(DecodeArgs a, int sms, cudaStream_t st) {
   a.rows_gu = ceil_div(a.I, sms) < 128 ? ceil_div(a.I, sms) : 128;
   // blocks of a group in the down projection: as many as its rows fit one tile, where K is long enough to cut (1 / 2 / 4
-  // blocks: 24 tokens x 2048 x 5632 39.6 / 35.7 / 34.2 us, 64 x 2048 x 8192 54.9 / 46.5 / 45.0)
+  // blocks: 24 tokens x 2048 x 5632 35.2 / 31.8 / 29.7 us, 64 x 2048 x 8192 50.8 / 42.6 / 40.3)
   a.ksplit = kMaxSplit;
   while (a.ksplit > 1 && (ceil_div(a.I, BK) < 8 * a.ksplit || 4 * ceil_div(a.H / 4, sms / a.ksplit) > BM || sms / a.ksplit > kMaxGroups)) a.ksplit /= 2;
   a.groups = sms / a.ksplit;
@@ -1260,10 +1261,10 @@ extern "C" int omni_decode(const void* x, const void* gate_w, const void* up_w, 
   a.partial = reinterpret_cast<float*>(w);
   a.y = static_cast<__nv_bfloat16*>(y), a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // The form.  Up to 8 tokens the direct one is the faster at every size (hidden x intermediate, direct / ring in us:
-  // 256 x 1024 13.8 / 17.5, 1024 x 4096 17.3 / 20.3, 2048 x 8192 31.8 / 33.1, 4096 x 11008 56.5 / 61.6).  From 9 to 16 it
-  // has half the weights in flight and loses once a block has much to stream (1024 x 4096, 0.17 MB a block, 18.7 / 20.6;
-  // 2048 x 5632, 0.48 MB, 31.4 / 28.0; 4096 x 11008 73.0 / 62.9); beyond, its token operand no longer fits the registers.
+  // The form.  Up to 8 tokens the direct one is the faster at every size (8 tokens, hidden x intermediate, direct / ring in us:
+  // 256 x 1024 13.6 / 17.6, 1024 x 4096 16.8 / 21.2, 2048 x 8192 30.3 / 32.3, 4096 x 11008 55.0 / 60.7).  From 9 to 16 it has
+  // half the weights in flight and loses once a block has much to stream (16 tokens: 1024 x 4096, 0.17 MB a block, 18.7 / 21.2;
+  // 2048 x 5632, 0.47 MB, 30.4 / 27.9; 4096 x 11008 72.1 / 62.5); beyond, its token operand no longer fits the registers.
   const int64_t bytes = 2 * (3 * static_cast<int64_t>(intermediate) + 2 * sqrt_n) * hidden;
   if (num_tokens <= 8) return launch_direct<1>(a, sms, st);
   if (num_tokens <= 16 && bytes <= sms * (int64_t(1) << 18)) return launch_direct<2>(a, sms, st);

@@ -359,7 +359,10 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const NormBwdArgs a) 
 // Many rows: the copy engine brings whole rows into a ring of shared-memory stages (rpc rows of h, dy and dh each), ahead
 // of the threads, so that the barrier of a row's sum leaves no gap in the traffic.  (16384 x 4096 bf16 with dh: rows into
 // registers 191 us, the next row's registers loaded ahead 140, ring 124, with two stages and a third block on the
-// multiprocessor 97 = 5.5 TB/s; a producer warp of its own for the copies gains nothing.)
+// multiprocessor 97 = 5.5 TB/s; a producer warp of its own for the copies gains nothing.
+// From kManyRows on: bf16, registers / ring, cold L2, in us: 1024 x 4096 22.9 / 21.5, 2048 x 4096 36 / 30, 4096 x 4096 54 / 40,
+// at 256 and 1024 columns the same within 2; below, 512 x 256 11.3 / 13.3.  In fp32 the ring is the slower at 4096 columns, 66 / 79
+// at 4096 rows, and the same within 2 at 256 and 1024.)
 constexpr int kBwdStages = 2;
 template <typename T, int VE, int V>
 __global__ void __launch_bounds__(512) rms_norm_bwd_ring_kernel(const NormBwdArgs a) {
@@ -551,8 +554,10 @@ void row_shape(int64_t T, int H, int per_thread, int& per, int& warps, int& rpc)
   rpc = warps >= 8 ? 1 : 8 / warps;
   if (T < rpc) rpc = static_cast<int>(T);
 }
-// Many rows: 16 values a thread (16384 x 4096 bf16 with residual and codes: 8 / 16 / 32 values 121 / 106 / 117 us); few
-// rows: 8, so that a row's loads are spread over more warps.  Rows that move value by value need an address each: 8 as well.
+// Many rows: 16 values a thread; few rows: 8, so that a row's loads are spread over more warps.  (Forward with residual and
+// codes, bf16, cold L2, 8 / 16 values in us: 16384 x 4096 117 / 97, 4096 x 4096 35.8 / 31.8, 2048 x 4096 22.4 / 19.4,
+// 1024 x 4096 15.3 / 15.4, 512 x 1024 8.6 / 9.2, 256 x 1024 7.2 / 9.2.  At other widths, 256 to 8192, and in fp32 the two are
+// within 2.5 us of one another, of 7 to 340, from 1024 rows on.)  Rows that move value by value need an address each: 8 as well.
 constexpr int kManyRows = 1024;
 
 template <typename T>
@@ -578,8 +583,11 @@ int launch_norm(const NormArgs& a0, cudaStream_t st) {
   return check_launch("rms_norm_kernel");
 }
 
-// As many blocks as a multiprocessor holds at 80 registers a thread (16384 x 4096 bf16, stages x blocks of 256 threads:
-// 3 x 2 124 us, 2 x 2 113, 2 x 3 103), fewer where a block would have less than four turns (each costs a partial row).
+// As many blocks as a multiprocessor holds at 80 registers a thread, which the ring's kernel has at 16 values of 16 bits
+// (16384 x 4096 bf16, stages x blocks of 256 threads, before the packed conversions: 3 x 2 124 us, 2 x 2 113, 2 x 3 103),
+// fewer where a block would have less than four turns (each costs a partial row).  Other instantiations are not as well
+// served: at 16 values of 32 bits (112 registers) two of the three are resident, and from 6145 columns on a block has more
+// than 384 threads, which leaves one.
 constexpr int kBwdBlocks = 3;
 int bwd_blocks(int64_t T, int rpc, int threads) {
   const int64_t turns = ceil_div64(T, rpc), sms = multiprocessors();

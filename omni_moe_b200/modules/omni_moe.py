@@ -448,10 +448,11 @@ class OmniMoE(nn.Module):
 
     def decode(self, hidden_states: torch.Tensor) -> torch.Tensor:
         """The eval-mode forward of at most 64 tokens ``[B, S, H]`` as one kernel (:func:`omni_decode_func`): the decode
-        steps of a serving program.  The same definition as :meth:`forward`, another order of summation.  Allocates
-        only its output (and a per-stream workspace once), so it can be captured in a CUDA graph, best after one call
-        outside it (the BatchNorm fold of the running statistics is then not part of the graph, and replays see the
-        statistics of the module's latest call); inference only."""
+        steps of a serving program.  The same definition as :meth:`forward`, another order of summation.  A bf16 module whose
+        sizes are multiples of 8 allocates only its output (and a per-stream workspace once); others copy all their weights
+        and tables in every call.  It can be captured in a CUDA graph, best after one call outside it (the BatchNorm fold of
+        the running statistics is then not part of the graph, and replays see the statistics of the module's latest call).
+        Inference only; ``last_routing`` is None afterwards, the selection stays in the kernel."""
         from ..ops.decode import omni_decode_func
         if self.training:
             raise RuntimeError("decode() uses the running statistics of the router's BatchNorm: call eval() first")

@@ -19,7 +19,8 @@ def scale_columns(cols: int) -> int:
 
 
 def mx_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """``(codes [rows, cols], scales [rows, ceil(cols / 32)])`` of a matrix (bf16, fp16 or fp32; rows may have a stride)."""
+    """``(codes [rows, cols], scales [rows, ceil(cols / 32)])`` of a matrix (bf16, fp16 or fp32; rows may have a stride).
+    The codes carry no gradient."""
     return _lib.binding().mx_quantize(x)
 
 
