@@ -208,8 +208,8 @@ class OmniMoE(nn.Module):
             return (self.router_norm_x.process_group,)
         return None
 
-    def _note_captured_step(self) -> None:
-        if torch.cuda.is_current_stream_capturing():
+    def _note_captured_step(self, t: torch.Tensor) -> None:
+        if t.is_cuda and torch.cuda.is_current_stream_capturing():
             self._bn_moved_by_graphs = True
 
     def _bn_fold_train(self, logits: torch.Tensor, b: "_Buffers | None" = None):
@@ -218,7 +218,7 @@ class OmniMoE(nn.Module):
         On one rank this is the library's kernel pair (no allocation, no host read: capturable); with
         synchronised statistics the per-rank moments are merged through torch.distributed."""
         n = self.num_expert_sqrt
-        self._note_captured_step()
+        self._note_captured_step(logits)
         grp = self._bn_group()
         bx, by = self.router_norm_x, self.router_norm_y
         run_dt = bx.running_mean.dtype if bx.running_mean is not None else torch.float32
@@ -405,7 +405,7 @@ class OmniMoE(nn.Module):
                                                         fold, self.training)
         else:
             if self.training:
-                self._note_captured_step()
+                self._note_captured_step(x)
             logits_x = self.router_norm_x(self.router_gate_x(x))
             logits_y = self.router_norm_y(self.router_gate_y(x))
             # log-probabilities, scores and routing weights stay in fp32 (the reference keeps the module dtype):

@@ -33,7 +33,8 @@ def omni_rms_norm_func(x: torch.Tensor, weight: torch.Tensor, residual: Optional
     :return: :class:`RmsNormOutput`
 
     Sums are fp32; rows may have any mean square that fp32 holds.  (With ``eps`` below 1e-30, rows whose root mean square is below
-    1e-17 leave fp32's normal range and lose precision, below 1e-19 all of it.)  Differentiable in ``x``, ``residual`` and ``weight``; the weight's gradient is summed in a fixed order.
+    1e-17 leave fp32's normal range and lose precision, below 1e-19 all of it.)  Differentiable in ``x``, ``residual`` and
+    ``weight``; the weight's gradient is summed in a fixed order.
     """
     refuse_tangents("omni_rms_norm_func", x, weight, residual)
     return RmsNormOutput(*_lib.binding().rms_norm(x, weight, residual, float(eps), bool(quantize), _lib.status_ptr(x)))
